@@ -1,0 +1,160 @@
+// Rows of keys and values into the 4-bit slot caches, and back (format: kv4.cuh).
+//
+// One thread per 8 dims: a 32-byte load, the group's extremes over 8 lanes, one 32-bit word of codes; lane 0 of a group stores
+// its (step, lo). A CTA takes a fixed range of channels over many rows, so that the channel's (layer, key | value, head) is
+// worked out once. What it has to move is the fp32 rows (8 times the codes), so it is bound by reading them.
+#include "kv4.cuh"
+
+using namespace b200dec_detail;
+
+namespace {
+
+struct Kv4Args {
+  float* kv;  // (nrows, layers * 2 * H * D)
+  const int* slot_of;
+  const int* frame_of;
+  uint32_t* ck;  // (L, S1, H, T, D / 8) words of codes
+  uint32_t* cv;
+  uint32_t* ckm;  // (L, S1, H, T, D / 64) {step, lo}
+  uint32_t* cvm;
+  int nrows, L, S1, H, D, T;
+};
+
+constexpr int THREADS = 256;
+
+struct f32x8 {
+  float v[8];
+};
+DEVI f32x8 ld_stream32(const float* p) {
+  f32x8 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(r.v[0]), "=f"(r.v[1]), "=f"(r.v[2]), "=f"(r.v[3]), "=f"(r.v[4]), "=f"(r.v[5]), "=f"(r.v[6]), "=f"(r.v[7])
+               : "l"(p));
+  return r;
+}
+DEVI void st32(float* p, const f32x8& r) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(r.v[0]), "f"(r.v[1]), "f"(r.v[2]), "f"(r.v[3]),
+               "f"(r.v[4]), "f"(r.v[5]), "f"(r.v[6]), "f"(r.v[7])
+               : "memory");
+}
+
+// the thread's 8 dims of every row: which layer, key or value, head and dim they belong to
+struct Channel {
+  int l, kvi, h, d8;
+  bool live;
+};
+DEVI Channel channel(const Kv4Args& p) {
+  const int d8n = p.D / 8, chunks = p.L * 2 * p.H * d8n;
+  const int c = blockIdx.x * THREADS + threadIdx.x, cc = min(c, chunks - 1);
+  return Channel{cc / (d8n * p.H * 2), (cc / (d8n * p.H)) & 1, (cc / d8n) % p.H, cc % d8n, c < chunks};
+}
+DEVI size_t vec_of(const Kv4Args& p, const Channel& c, int slot, int frame) {
+  return (((size_t)c.l * p.S1 + slot) * p.H + c.h) * p.T + frame;
+}
+DEVI bool inside(const Kv4Args& p, int slot, int frame) { return slot >= 0 && slot < p.S1 && frame >= 0 && frame < p.T; }
+
+__global__ void __launch_bounds__(THREADS) scatter_kv_q4_kernel(const Kv4Args p) {
+  const Channel c = channel(p);
+  const size_t width = (size_t)p.L * 2 * p.H * p.D, at = (size_t)(blockIdx.x * THREADS + threadIdx.x) * 8;
+  for (int row = blockIdx.y; row < p.nrows; row += gridDim.y) {
+    const int slot = __ldg(p.slot_of + row), frame = __ldg(p.frame_of + row);
+    if (!inside(p, slot, frame)) continue;  // the whole CTA
+    f32x8 x{};
+    if (c.live) x = ld_stream32(p.kv + row * width + at);
+    float mn = INFINITY, mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const uint32_t w = pack_bf16(x.v[i], x.v[i + 1]);
+      x.v[i] = kv4_clamp(bf16_lo(w)), x.v[i + 1] = kv4_clamp(bf16_hi(w));
+      mn = fminf(mn, fminf(x.v[i], x.v[i + 1])), mx = fmaxf(mx, fmaxf(x.v[i], x.v[i + 1]));
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    if (!c.live) continue;
+    const Kv4Group g = kv4_group(mn, mx);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= (uint32_t)kv4_code(x.v[i], g) << (4 * i);
+    const size_t vec = vec_of(p, c, slot, frame);
+    (c.kvi ? p.cv : p.ck)[vec * (p.D / 8) + c.d8] = w;
+    if ((c.d8 & 7) == 0) (c.kvi ? p.cvm : p.ckm)[vec * (p.D / 64) + (c.d8 >> 3)] = g.word;
+  }
+}
+
+__global__ void __launch_bounds__(THREADS) gather_kv_q4_kernel(const Kv4Args p) {
+  const Channel c = channel(p);
+  if (!c.live) return;
+  const size_t width = (size_t)p.L * 2 * p.H * p.D, at = (size_t)(blockIdx.x * THREADS + threadIdx.x) * 8;
+  for (int row = blockIdx.y; row < p.nrows; row += gridDim.y) {
+    const int slot = __ldg(p.slot_of + row), frame = __ldg(p.frame_of + row);
+    f32x8 x{};
+    if (inside(p, slot, frame)) {
+      const size_t vec = vec_of(p, c, slot, frame);
+      const uint32_t w = (c.kvi ? p.cv : p.ck)[vec * (p.D / 8) + c.d8];
+      const uint32_t m = (c.kvi ? p.cvm : p.ckm)[vec * (p.D / 64) + (c.d8 >> 3)];
+      const float step = __half2float(__ushort_as_half(m & 0xffff)), lo = __half2float(__ushort_as_half(m >> 16));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.v[i] = kv4_value((w >> (4 * i)) & 15, step, lo);
+    }
+    st32(p.kv + row * width + at, x);
+  }
+}
+
+int check_kv4(const char* what, const void* kv, const int32_t* slot_of, const int32_t* frame_of, const void* ck, const void* cv,
+              const void* ckm, const void* cvm, int nrows, int layers, int slots_plus_1, int heads, int head_dim, int frames) {
+  B200_REQUIRE(nrows >= 0, "%s: nrows %d", what, nrows);
+  B200_REQUIRE(kv && slot_of && frame_of && ck && cv && ckm && cvm, "%s: null pointer", what);
+  B200_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim %d (64 or 128)", what, head_dim);
+  B200_REQUIRE(layers >= 1 && slots_plus_1 >= 1 && heads >= 1 && frames >= 1 && (int64_t)layers * 2 * heads * head_dim <= 1 << 28,
+               "%s: layers %d slots %d heads %d frames %d", what, layers, slots_plus_1, heads, frames);
+  B200_REQUIRE(((uintptr_t)kv & 31) == 0 && (((uintptr_t)ck | (uintptr_t)cv | (uintptr_t)ckm | (uintptr_t)cvm) & 3) == 0,
+               "%s: alignment (the rows 32 bytes, the caches 4)", what);
+  return 0;
+}
+
+dim3 kv4_grid(const Kv4Args& p) {
+  const int x = (p.L * 2 * p.H * (p.D / 8) + THREADS - 1) / THREADS;
+  const int y = (148 * 8 * 4 + x - 1) / x;  // about four waves of CTAs
+  return dim3(x, p.nrows < y ? p.nrows : y);
+}
+
+Kv4Args kv4_args(float* kv, const int32_t* slot_of, const int32_t* frame_of, void* ck, void* cv, void* ckm, void* cvm, int nrows,
+                 int layers, int slots_plus_1, int heads, int head_dim, int frames) {
+  return Kv4Args{kv, slot_of, frame_of, (uint32_t*)ck, (uint32_t*)cv, (uint32_t*)ckm, (uint32_t*)cvm, nrows, layers, slots_plus_1,
+                 heads, head_dim, frames};
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200dec_scatter_kv_q4(const float* kv, const int32_t* slot_of, const int32_t* frame_of, void* ck, void* cv, void* ck_pairs,
+                          void* cv_pairs, int nrows, int layers, int slots_plus_1, int heads, int head_dim, int frames,
+                          void* stream) {
+  if (const int rc = check_kv4("scatter_kv_q4", kv, slot_of, frame_of, ck, cv, ck_pairs, cv_pairs, nrows, layers, slots_plus_1,
+                               heads, head_dim, frames))
+    return rc;
+  if (nrows == 0) return 0;
+  const Kv4Args p = kv4_args(const_cast<float*>(kv), slot_of, frame_of, ck, cv, ck_pairs, cv_pairs, nrows, layers, slots_plus_1,
+                             heads, head_dim, frames);
+  scatter_kv_q4_kernel<<<kv4_grid(p), THREADS, 0, (cudaStream_t)stream>>>(p);
+  return check_launch("scatter_kv_q4");
+}
+
+int b200dec_gather_kv_q4(float* kv, const int32_t* slot_of, const int32_t* frame_of, const void* ck, const void* cv,
+                         const void* ck_pairs, const void* cv_pairs, int nrows, int layers, int slots_plus_1, int heads,
+                         int head_dim, int frames, void* stream) {
+  if (const int rc = check_kv4("gather_kv_q4", kv, slot_of, frame_of, ck, cv, ck_pairs, cv_pairs, nrows, layers, slots_plus_1,
+                               heads, head_dim, frames))
+    return rc;
+  if (nrows == 0) return 0;
+  const Kv4Args p = kv4_args(kv, slot_of, frame_of, const_cast<void*>(ck), const_cast<void*>(cv), const_cast<void*>(ck_pairs),
+                             const_cast<void*>(cv_pairs), nrows, layers, slots_plus_1, heads, head_dim, frames);
+  gather_kv_q4_kernel<<<kv4_grid(p), THREADS, 0, (cudaStream_t)stream>>>(p);
+  return check_launch("gather_kv_q4");
+}
+
+}  // extern "C"

@@ -1,0 +1,48 @@
+// The 4-bit cache format, shared by everything that writes it (kv4.cu, attention_q4.cu, prefill_gemm.cu).
+//
+// A head vector is rounded to bf16 (what the bf16 cache would hold), clamped to +-32752 with NaN as 0, and cut into groups of
+// 64 dims. Per group: lo = fp16(min), step = fp16((max - lo) / 15), code = clamp(rint((x - lo) / step), 0, 15), 0 where step
+// is 0; x ~ lo + code * step. Within half a step, except that rounding lo and step to 11 bits can move a value by
+// 2^-12 (|lo| + range) more. The clamp keeps max - min inside fp16. 64 dims share a (step, lo) pair of 4 bytes: 4.5 bits a value.
+// A vector's codes are D / 2 bytes, dim 2i in the low half of byte i; its pairs are D / 64 half2 {step, lo}.
+#pragma once
+#include "common.cuh"
+
+namespace b200dec_detail {
+
+constexpr float KV4_LIMIT = 32752.f;
+
+// x as the format sees it, for values already rounded to bf16
+DEVI float kv4_clamp(float x) { return x != x ? 0.f : fminf(fmaxf(x, -KV4_LIMIT), KV4_LIMIT); }
+
+struct Kv4Group {
+  float lo, step, inv;
+  uint32_t word;  // half2 {step, lo}
+};
+DEVI Kv4Group kv4_group(float mn, float mx) {
+  Kv4Group g;
+  const __half lo = __float2half_rn(mn);
+  g.lo = __half2float(lo);
+  const __half step = __float2half_rn(__fdiv_rn(mx - g.lo, 15.f));
+  g.step = __half2float(step);
+  g.inv = g.step > 0.f ? __frcp_rn(g.step) : 0.f;
+  g.word = (uint32_t)__half_as_ushort(step) | ((uint32_t)__half_as_ushort(lo) << 16);
+  return g;
+}
+
+// rint((x - lo) / step) clamped to 0..15, as if the quotient were exact: the product with the reciprocal is off by a few
+// 2^-23, so its rounding can only be wrong beside a half; the remainder d - c * step is exact (c has 4 bits, step 11), and
+// against half a step it decides, ties to even. (x - lo itself is exact for bf16 x and fp16 lo unless one is 2^13 times
+// smaller than the other; then the difference is correctly rounded.)
+DEVI int kv4_code(float x, const Kv4Group& g) {
+  const float d = x - g.lo;
+  float c = fminf(fmaxf(rintf(d * g.inv), 0.f), 15.f);
+  const float e2 = 2.f * __fmaf_rn(-c, g.step, d);
+  const bool odd = ((int)c & 1) != 0;
+  if (e2 > g.step || (e2 == g.step && odd)) c += 1.f;
+  if (-e2 > g.step || (-e2 == g.step && odd)) c -= 1.f;
+  return g.step > 0.f ? (int)fminf(fmaxf(c, 0.f), 15.f) : 0;
+}
+DEVI float kv4_value(int code, float step, float lo) { return __fmaf_rn((float)code, step, lo); }
+
+}  // namespace b200dec_detail

@@ -53,6 +53,7 @@ int b200dec_sizeof(int which) {
     case 2: return (int)sizeof(b200dec_layer);
     case 3: return (int)sizeof(b200dec_plan);
     case 4: return (int)sizeof(b200dec_ln_link);
+    case 5: return (int)sizeof(b200dec_rules);
   }
   return -1;
 }

@@ -18,7 +18,8 @@ W_BF16, W_INT8, W_INT8_24, W_INT8_UMMA, W_F16, W_F16_UMMA, W_INT8_24_UMMA = 0, 1
 A_F16, A_F32_SPLIT, A_F16_ROWS16 = 0, 1, 2
 OUT_F16, OUT_F32, OUT_F32_ADD = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
-ST_TOKEN_RANGE, ST_POS_RANGE, ST_FRAMES_RANGE, ST_SLOT_RANGE, ST_TIMEOUT = 1, 2, 4, 8, 16
+T_F32, T_F16, T_BF16 = 0, 1, 2
+ST_TOKEN_RANGE, ST_POS_RANGE, ST_FRAMES_RANGE, ST_SLOT_RANGE, ST_TIMEOUT, ST_NO_TOKEN = 1, 2, 4, 8, 16, 32
 PREFILL_HIGH_ROWS = 8
 
 vp, i32, i64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
@@ -58,6 +59,11 @@ class Plan(C.Structure):
                 ("attn_part", vp), ("attn_count", vp), ("head_max", vp), ("head_idx", vp),
                 ("xh", vp), ("ln_stats", vp), ("sched_self", vp), ("sched_cross", vp), ("logits", vp), ("argmax", vp),
                 ("fused_ws", vp * 16)]
+
+
+class Rules(C.Structure):
+    _fields_ = [("params", vp), ("history", vp), ("last", vp), ("plen", vp), ("bias_ids", vp), ("bias", vp), ("bias_n", vp),
+                ("mask", vp), ("mask_on", vp), ("hist_cols", i32), ("max_bias", i32)]
 
 
 # name -> (restype, argtypes); every symbol include/b200dec.h declares
@@ -114,6 +120,20 @@ PROTOTYPES = {
                                          vp, C.c_int, C.c_int, vp, vp, vp, C.c_int, vp]),
     "b200dec_attention_static": (C.c_int, [C.c_int, vp, vp, C.c_int, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int,
                                            f32, vp, C.c_int, C.c_int, vp, C.c_int, vp]),
+    "b200dec_attention_q4": (C.c_int, [C.c_int, vp, vp, C.c_int, vp, vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int,
+                                       f32, vp, C.c_int, C.c_int, vp, vp, vp, C.c_int, vp]),
+    "b200dec_attention_q4_scratch_floats": (i64, [C.c_int] * 4),
+    "b200dec_scatter_kv_q4": (C.c_int, [vp] * 7 + [C.c_int] * 6 + [vp]),
+    "b200dec_gather_kv_q4": (C.c_int, [vp] * 7 + [C.c_int] * 6 + [vp]),
+    "b200dec_logit_rules": (C.c_int, [vp, C.c_int, i64, C.c_int, C.c_int, vp, C.c_int, C.POINTER(Rules), vp, i64, vp, vp, vp,
+                                      C.c_int, vp]),
+    "b200dec_w8a8_rows_bytes": (i64, [C.c_int, C.c_int]),
+    "b200dec_w8a8_weight_bytes": (i64, [C.c_int, C.c_int]),
+    "b200dec_w8a8_pack_rows": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, i64, vp, vp, vp]),
+    "b200dec_w8a8_tile_weight": (C.c_int, [vp, C.c_int, C.c_int, vp, vp]),
+    "b200dec_w8a8_linear": (C.c_int, [vp, vp, C.c_int, C.c_int, vp, vp, vp, C.c_int, C.c_int, vp, C.c_int, i64, vp, vp]),
+    "b200dec_w8a8_prefill": (C.c_int, [vp, vp, C.c_int, C.c_int, vp, vp, vp, C.c_int, C.c_int, vp, C.c_int, vp, vp, vp, vp,
+                                       C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp]),
     "b200dec_scatter_kv": (C.c_int, [vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp]),
     "b200dec_prefill_rows_bytes": (i64, [C.c_int, C.c_int]),
     "b200dec_prefill_pack_rows": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, vp, vp]),
@@ -149,7 +169,7 @@ def lib() -> C.CDLL:
         for name, (res, args) in PROTOTYPES.items():
             fn = getattr(handle, name)
             fn.restype, fn.argtypes = res, args
-        for which, struct in enumerate((Weight, Norm, Layer, Plan, LnLink)):  # this binding against the built library
+        for which, struct in enumerate((Weight, Norm, Layer, Plan, LnLink, Rules)):  # this binding against the built library
             if handle.b200dec_sizeof(which) != C.sizeof(struct):
                 raise NativeError(f"{struct.__name__}: {C.sizeof(struct)} bytes here, {handle.b200dec_sizeof(which)} "
                                   f"in {LIB_PATH}: rebuild the library (build.py --force)")
@@ -167,6 +187,13 @@ def ptr(t: torch.Tensor | None) -> int | None:
         return None
     assert t.is_cuda and t.is_contiguous(), "device-resident contiguous tensors only"
     return t.data_ptr()
+
+
+def image(n: int, device) -> torch.Tensor:
+    """n bytes on a 1 KB boundary (the swizzle atom of the tile images; the allocator gives 512)."""
+    buf = torch.empty(n + 1024, dtype=torch.uint8, device=device)
+    at = -buf.data_ptr() % 1024
+    return buf[at:at + n]
 
 
 def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:

@@ -200,3 +200,69 @@ def dequantized(weight: torch.Tensor, kind: int) -> torch.Tensor:
         w = prune_24_magnitude(w)
     q, s = quantize_rows(w)
     return q.float() * s[:, None]
+
+
+class W8A8Linear:
+    """A projection multiplied in 8-bit integers on the tcgen05 tensor cores: y = act((q_x q_w^T) * s_x * s_w + bias) with rows
+    quantised as they come, one scale each. The form for many rows (encoder frames, whole sentences); the decoding step's
+    projections keep 16-bit rows (PackedLinear). q: int8 (n, k) and scale: fp32 (n,) as quantize_rows gives them, bias: (n,)
+    or None. Holds its own copies; a call allocates what it needs on the current stream, so calls on several streams and
+    inside a capture are like any other torch operation's."""
+
+    ACTS = {None: nv.ACT_NONE, "relu": nv.ACT_RELU, "gelu": nv.ACT_GELU}
+    KINDS = {torch.float32: nv.T_F32, torch.float16: nv.T_F16, torch.bfloat16: nv.T_BF16}
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None):
+        if not (q.is_cuda and q.dtype == torch.int8 and q.dim() == 2 and q.numel()):
+            raise ValueError("W8A8Linear: q must be a non-empty int8 (n, k) matrix on a CUDA device")
+        self.n, self.k, self.device, self.act = int(q.shape[0]), int(q.shape[1]), q.device, self.ACTS[act]
+        if scale.shape != (self.n,) or (bias is not None and bias.shape != (self.n,)):
+            raise ValueError("W8A8Linear: one scale (and bias) per channel")
+        lib = nv.lib()
+        size = lib.b200dec_w8a8_weight_bytes(self.n, self.k)
+        if size < 0:
+            raise ValueError(f"W8A8Linear: k = {self.k} is beyond the 32-bit sums")
+        with torch.cuda.device(self.device):
+            self.scale = scale.detach().to(self.device, torch.float32).contiguous().clone()
+            self.bias = None if bias is None else bias.detach().to(self.device, torch.float32).contiguous().clone()
+            self.image = nv.image(size, self.device)
+            self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+            q = q.contiguous()
+            nv.check(lib.b200dec_w8a8_tile_weight(nv.ptr(q), self.n, self.k, nv.ptr(self.image), nv.stream_ptr()))
+            torch.cuda.current_stream().synchronize()  # any stream may use the image from now on
+
+    @classmethod
+    def from_weight(cls, w: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None) -> "W8A8Linear":
+        """The weight (n, k) quantised by quantize_rows."""
+        return cls(*quantize_rows(w), bias, act)
+
+    def _rows(self, x: torch.Tensor) -> tuple[int, torch.Tensor, int, int]:
+        """Checks x (m, k), quantises its rows on the current stream: m, the work buffer, the image's and the scales' address."""
+        if not (x.device == self.device and x.dim() == 2 and x.shape[1] == self.k and x.dtype in self.KINDS):
+            raise ValueError(f"W8A8Linear: rows of {self.k} fp32, fp16 or bf16 values on {self.device}")
+        if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < self.k):
+            x = x.contiguous()
+        m, lib = int(x.shape[0]), nv.lib()
+        size = lib.b200dec_w8a8_rows_bytes(m, self.k)
+        work = torch.empty(1024 + size + 4 * m, dtype=torch.uint8, device=self.device)
+        image = work.data_ptr() + -work.data_ptr() % 1024
+        if m:
+            nv.check(lib.b200dec_w8a8_pack_rows(x.data_ptr(), self.KINDS[x.dtype], m, self.k, x.stride(0), image, image + size,
+                                                nv.stream_ptr()))
+        return m, work, image, image + size
+
+    def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """x (m, k) fp32, fp16 or bf16, rows any distance apart -> (m, n) of x's type (or dtype, or into out, rows any distance
+        apart)."""
+        if out is None:
+            out = torch.empty(x.shape[0], self.n, dtype=dtype or x.dtype, device=self.device)
+        if not (out.device == self.device and out.shape == (x.shape[0], self.n) and out.dtype in self.KINDS and out.stride(1) == 1
+                and (out.shape[0] <= 1 or out.stride(0) >= self.n) and dtype in (None, out.dtype)):
+            raise ValueError(f"W8A8Linear: out must be ({x.shape[0]}, {self.n}) fp32, fp16 or bf16 with dense rows on {self.device}")
+        with torch.cuda.device(self.device):
+            m, work, image, scales = self._rows(x)
+            if m:
+                nv.check(nv.lib().b200dec_w8a8_linear(image, scales, m, self.k, nv.ptr(self.image), nv.ptr(self.scale),
+                                                      nv.ptr(self.bias), self.n, self.act, out.data_ptr(), self.KINDS[out.dtype],
+                                                      out.stride(0), nv.ptr(self.status), nv.stream_ptr()))
+        return out

@@ -34,13 +34,6 @@ def _fp32(t: torch.Tensor) -> torch.Tensor:
     return t.detach().float().contiguous()
 
 
-def _image(n: int, device) -> torch.Tensor:
-    """n bytes on a 1 KB boundary (the swizzle atom of the tile images; the allocator gives 512)."""
-    buf = torch.empty(n + 1024, dtype=torch.uint8, device=device)
-    at = -buf.data_ptr() % 1024
-    return buf[at:at + n]
-
-
 class _Layer:
     """One decoder layer as the step's kernels read it: six packed projections (q, k and v fused into one, as the
     reference fuses them, kernels/stream_decoder.py:56-57) and the three LayerNorms in fp32. The projections that
@@ -87,7 +80,7 @@ class _PrefillWeight:
         self.n, self.k = -(-n // 256) * 256, k
         wb = torch.zeros(self.n, k, dtype=torch.bfloat16, device=w.device)
         wb[:n] = w.detach().to(torch.bfloat16)
-        self.image = _image(self.n * k * 2, w.device)
+        self.image = nv.image(self.n * k * 2, w.device)
         nv.check(nv.lib().b200dec_prefill_tile_weight(nv.ptr(wb), self.n, k, nv.ptr(self.image), nv.stream_ptr()))
         torch.cuda.current_stream().synchronize()
         self.bias = torch.zeros(self.n, device=w.device)
@@ -307,7 +300,7 @@ class StreamDecoder:
         self.head = packed("head")
         for name in ("proj", "cross"):
             w = object.__new__(_PrefillWeight)
-            w.image, w.bias = _image(t[f"prefill.{name}.image"].numel(), self.device), t[f"prefill.{name}.bias"]
+            w.image, w.bias = nv.image(t[f"prefill.{name}.image"].numel(), self.device), t[f"prefill.{name}.bias"]
             w.image.copy_(t[f"prefill.{name}.image"])
             w.n, w.k = manifest["prefill"][name]
             setattr(self, name, w)

@@ -41,11 +41,13 @@ enum { B200DEC_A_F16 = 0, B200DEC_A_F32_SPLIT = 1,  /* activation operand of a p
                                       (see b200dec_ln_link) */
 enum { B200DEC_OUT_F16 = 0, B200DEC_OUT_F32 = 1, B200DEC_OUT_F32_ADD = 2 };/* store, or add into an fp32 residual */
 enum { B200DEC_ACT_NONE = 0, B200DEC_ACT_RELU = 1, B200DEC_ACT_GELU = 2 };
+enum { B200DEC_T_F32 = 0, B200DEC_T_F16 = 1, B200DEC_T_BF16 = 2 };  /* element type of a tensor handed to the calls that take one */
 enum { B200DEC_OK = 0, B200DEC_EINVAL = 1, B200DEC_ECUDA = 2, B200DEC_EARCH = 3 };
 
 /* bits of the device status word (written by kernels, never cleared by them) */
 enum { B200DEC_ST_TOKEN_RANGE = 1, B200DEC_ST_POS_RANGE = 2, B200DEC_ST_FRAMES_RANGE = 4, B200DEC_ST_SLOT_RANGE = 8,
-       B200DEC_ST_TIMEOUT = 16 /* a bounded wait inside a kernel ran out; the kernel returned without its result */ };
+       B200DEC_ST_TIMEOUT = 16 /* a bounded wait inside a kernel ran out; the kernel returned without its result */,
+       B200DEC_ST_NO_TOKEN = 32 /* the rules left a row no token (b200dec_logit_rules): token 0 was taken */ };
 
 /* One projection y = a W^T (* scale) + bias in the tiled layout. */
 typedef struct b200dec_weight {
@@ -154,7 +156,7 @@ typedef struct b200dec_plan {
 const char* b200dec_last_error(void);
 int b200dec_version(void);
 /* sizeof the structures above as this library was compiled (which: 0 b200dec_weight, 1 b200dec_norm, 2 b200dec_layer,
- * 3 b200dec_plan, 4 b200dec_ln_link), so that a binding in another language can check its own layout. */
+ * 3 b200dec_plan, 4 b200dec_ln_link, 5 b200dec_rules), so that a binding in another language can check its own layout. */
 int b200dec_sizeof(int which);
 
 /* ---- packing (init time) ------------------------------------------------------------------------------------ */
@@ -338,6 +340,83 @@ int b200dec_scatter_kv(const float* kv, const int32_t* slot_of, const int32_t* f
 int b200dec_scatter_kv_q8(const float* kv, const int32_t* slot_of, const int32_t* frame_of, void* ck, void* cv,
                           float* ck_scale, float* cv_scale, int nrows, int layers, int slots_plus_1, int heads,
                           int head_dim, int frames, void* stream);
+/* ---- 4-bit caches ---------------------------------------------------------------------------------------------------
+ * A head vector is rounded to bf16, clamped to +-32752 (NaN as 0) and cut into groups of 64 dims; per group lo = fp16(min),
+ * step = fp16((max - lo) / 15), code = clamp(rint((x - lo) / step), 0, 15), 0 where step is 0; x ~ lo + code * step. Codes:
+ * uint8 (slots + 1, H, cap, D / 2), dim 2i in the low half of byte i. Pairs: fp16 (slots + 1, H, cap, D / 64, 2) = {step,
+ * lo}. 4.5 bits a value. head_dim 64 or 128. No counterpart in the reference. */
+/* b200dec_attention over 4-bit caches, for any cap: heads x head_dim as the caches have them, n[s] = 0 .. cap - 1 cached keys
+ * (self != 0: the row's new key and value are written at n[s] and attended in this step as bf16 values) or 0 .. cap frames
+ * (a row without any gives zeros). Scores, softmax and sums in fp32. sched: NULL, or a table of b200dec_row_schedule
+ * (16-byte aligned; active, n and status are then not read). part, count: a workspace of
+ * b200dec_attention_q4_scratch_floats() floats and rows * heads counters, zero on entry and on exit, for the calls of one
+ * stream at a time (two captured graphs that may run side by side need one each); both NULL: a row is one CTA however
+ * long it is. Two rows of one call must not append to the same slot, the dummy excepted. */
+int b200dec_attention_q4(int self, const int32_t* active, const float* q, int ldq, void* kcache, void* vcache, void* kpairs,
+                         void* vpairs, const int32_t* n, const int32_t* sched, int slots, int heads, int head_dim, int cap,
+                         float scale, void* out, int out_kind, int rows, float* part, int32_t* count, int32_t* status, int pdl,
+                         void* stream);
+int64_t b200dec_attention_q4_scratch_floats(int rows, int heads, int head_dim, int cap);
+/* b200dec_scatter_kv into 4-bit caches: kv (nrows, L * 2 * H * D) fp32, 32-byte aligned; codes (L, slots + 1, H, frames,
+ * D / 2), pairs (L, slots + 1, H, frames, D / 64, 2). Rows whose slot or frame is outside the caches are dropped; no two rows
+ * may have the same slot and frame. */
+int b200dec_scatter_kv_q4(const float* kv, const int32_t* slot_of, const int32_t* frame_of, void* ck, void* cv, void* ck_pairs,
+                          void* cv_pairs, int nrows, int layers, int slots_plus_1, int heads, int head_dim, int frames,
+                          void* stream);
+/* The way back: kv (nrows, L * 2 * H * D) fp32 = the values that the caches hold for frame frame_of[i] of slot slot_of[i]
+ * (zeros where that is outside them). */
+int b200dec_gather_kv_q4(float* kv, const int32_t* slot_of, const int32_t* frame_of, const void* ck, const void* cv,
+                         const void* ck_pairs, const void* cv_pairs, int nrows, int layers, int slots_plus_1, int heads,
+                         int head_dim, int frames, void* stream);
+/* ---- rules on the logits ----------------------------------------------------------------------------------------------
+ * What a slot's request asks of the choice of its tokens; every table has slots + 1 rows, in device memory. */
+typedef struct b200dec_rules {
+  const float* params;     /* (slots + 1, 4), 16-byte aligned: repetition penalty (> 0; 1: none), presence penalty, frequency
+                              penalty (0: none), unused */
+  const int64_t* history;  /* (slots + 1, hist_cols): the slot's tokens; ids outside the vocabulary count for nothing */
+  const int32_t* last;     /* (slots + 1): history[0 .. last] counts (-1: none), last < hist_cols */
+  const int32_t* plen;     /* (slots + 1): history[plen .. last] are generated, what is before them is the prompt */
+  const int32_t* bias_ids; /* NULL (with the next two), or (slots + 1, max_bias) token ids, */
+  const float* bias;       /* what is added to their logits (-INFINITY bans a token; one listed twice gets both), */
+  const int32_t* bias_n;   /* and how many of a slot's entries count */
+  const uint32_t* mask;    /* NULL, or (slots + 1, (vocab + 31) / 32): bit v % 32 of word v / 32 set = token v is allowed */
+  const uint8_t* mask_on;  /* NULL: every slot has a mask; else (slots + 1), 0: the slot's mask is not looked at */
+  int32_t hist_cols, max_bias;  /* max_bias <= 1024 */
+} b200dec_rules;
+/* The greedy choice of every row under its slot's rules, slot = active[r]. With x a token's logit (fp32, fp16 or bf16 by
+ * kind, row r at logits + r * ldl): x = x > 0 ? x / repetition : x * repetition where the token is in the slot's history,
+ * then x - frequency * (times generated) - presence where it was generated, then x + its biases, then -INFINITY where the
+ * mask leaves it out; in fp32. token[r] = the first index of the largest (NaN is never chosen), best[r] (or NULL) its value;
+ * where nothing is above -INFINITY, token 0, and B200DEC_ST_NO_TOKEN for a slot that is not the dummy. out: NULL, or
+ * (rows, ldo) of kind, the logits under the rules (may be logits itself, with ldo = ldl). best and token are what b200dec_pick
+ * takes as one partial per row. No counterpart in the reference, whose choice is the plain argmax
+ * (kernels/csrc/decoder_ops.cu:106-147). */
+int b200dec_logit_rules(const void* logits, int kind, int64_t ldl, int rows, int vocab, const int32_t* active, int slots,
+                        const b200dec_rules* rules, void* out, int64_t ldo, float* best, int32_t* token, int32_t* status, int pdl,
+                        void* stream);
+/* ---- a product of 8-bit integers on the tcgen05 tensor cores -----------------------------------------------------------
+ * out (m, n) = act((q w^T) * row scale * channel scale + bias): rows quantised as they come, one scale each (s = max(max |x|,
+ * 1e-12) / 127, q = rint(x / s), NaN for a row that holds an infinity or NaN), int8 weights with one scale per channel
+ * (b200dec_quantize_rows), exact 32-bit sums, every later operation rounded once in fp32. Any m, n; k <= 131072. The operands
+ * are images of their shared-memory tiles, 1 KB aligned. The reference multiplies int8 weights with 16-bit rows
+ * (kernels/csrc/dec_w8.cu:46-234), as b200dec_linear does; this is the form for many rows. */
+int64_t b200dec_w8a8_rows_bytes(int m, int k);
+int64_t b200dec_w8a8_weight_bytes(int n, int k);
+/* x (m, ldx) of kind (B200DEC_T_*) -> image, scale (m). */
+int b200dec_w8a8_pack_rows(const void* x, int kind, int m, int k, int64_t ldx, void* image, float* scale, void* stream);
+/* q (n, k) int8 row-major -> image; init time. */
+int b200dec_w8a8_tile_weight(const int8_t* q, int n, int k, void* image, void* stream);
+/* w_scale (n) and bias (n) or NULL 16-byte aligned, act B200DEC_ACT_*, out (m, ldo) of out_kind (B200DEC_T_*). status receives
+ * B200DEC_ST_TIMEOUT if a bounded wait inside the kernel ran out. */
+int b200dec_w8a8_linear(const void* rows_image, const float* row_scale, int m, int k, const void* weight_image,
+                        const float* w_scale, const float* bias, int n, int act, void* out, int out_kind, int64_t ldo,
+                        int32_t* status, void* stream);
+/* The same product into the slot caches: mode, pieces and caches as b200dec_prefill_gemm (mode 3: 4-bit caches, with their
+ * pairs for ck_scale and cv_scale). */
+int b200dec_w8a8_prefill(const void* rows_image, const float* row_scale, int m, int k, const void* weight_image,
+                         const float* w_scale, const float* bias, int n, int mode, const int32_t* pieces, int n_pieces, void* ck,
+                         void* cv, void* ck_scale, void* cv_scale, int layers, int slots_plus_1, int heads, int head_dim, int frames,
+                         int32_t* status, void* stream);
 /* A measurement aid, no counterpart in the reference and not a step of the decoder: `ctas` CTAs of 128 threads each
  * read `bytes_per_cta` contiguous bytes of src (CTA c from src + c * bytes_per_cta) with the attention kernels' loads
  * (16 bytes per thread, streaming, 8 in flight) and do nothing else. The time of such a launch is what a kernel of
@@ -367,6 +446,7 @@ int b200dec_prefill_tile_weight(const void* w_bf16, int n, int k, void* image, v
  *   frames, head_dim) of keys (kv = 0) or values. Rows outside every piece or past the cache are dropped.
  * mode 2: the same into int8 caches with one fp32 scale per head vector (layers, slots_plus_1, heads, frames),
  *   quantised as b200dec_scatter_kv_q8 does.
+ * mode 3: the same into 4-bit caches, as b200dec_scatter_kv_q4 does; ck_scale and cv_scale are their fp16 pairs.
  * mode | B200DEC_PREFILL_HIGH_ROWS: the low halves of A are zero and the image does not hold them.
  * status receives B200DEC_ST_TIMEOUT if a bounded wait inside the kernel ran out. */
 #define B200DEC_PREFILL_HIGH_ROWS 8
