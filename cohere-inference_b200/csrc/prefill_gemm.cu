@@ -19,43 +19,38 @@
 //     (a thread owns one frame = one tensor-memory lane) while the next tile multiplies.
 //   * epilogues: (0) the result, split again into bf16 halves, in the operand image of the next product; (1) a head
 //     vector of D consecutive channels = 128 / 256 contiguous bytes of the bf16 cache row of (layer, slot, head,
-//     frame); (2) the same quantised as the reference's dec_scatter_kv_q8 does (bf16-round, absmax / 127, rint). The
+//     frame); (2) the same quantised as the reference's dec_scatter_kv_q8 does (bf16-round, absmax / 127, rint); (3) the same in
+//     4 bits (kv4.cuh). The
 //     frame's slot and index come from a table of pieces (first row, frames, slot) by binary search.
 // Every mbarrier wait is bounded; a wait that runs out sets B200DEC_ST_TIMEOUT, the roles fall through, copies in
 // flight are awaited (bounded) and tensor memory is released.
-#include <type_traits>
-
-#include "kv4.cuh"
+#include "kv_store.cuh"
+#include "umma.cuh"
 
 using namespace b200dec_detail;
 
 namespace {
 
-constexpr int BM = 128, BN = 256, BK = 64;
-constexpr int A_STAGE = BM * BK * 2, B_BLOCK = BN * BK * 2;
+constexpr int BM = UMMA_BM, BN = UMMA_BN, BK = 64;
 // TN: channels of a CTA's tile. 256, or 64 (a quarter of a weight block: 64 rows of 128 bytes, contiguous) where that
 // still is one wave.
-// I8: 8-bit integer operands (128 k to a block of 128 bytes), 32-bit integer accumulators, one copy of the rows.
-template <int TN, bool I8>
+template <int TN>
 struct Tile {
-  static constexpr int A_BYTES = (I8 ? 1 : 2) * A_STAGE, B_STAGE = TN * BK * 2, STAGE_BYTES = A_BYTES + B_STAGE;
-  static constexpr int STAGES = I8 ? (TN == BN ? 4 : TN == 128 ? 6 : 8) : TN == BN ? 3 : 5;
+  static constexpr int STAGES = TN == BN ? 3 : 5, B_STAGE = TN * BK * 2, STAGE_BYTES = 2 * A_STAGE + B_STAGE;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;  // slack to align the base to a swizzle atom
   static constexpr int TMEM_COLS = 2 * TN;                        // two accumulators
-  // bf16 x bf16 -> fp32, or signed 8-bit x signed 8-bit -> 32-bit; both operands K-major, M = 128, N = TN
+  // bf16 x bf16 -> fp32, both operands K-major, M = 128, N = TN
   static constexpr uint32_t IDESC =
-      ((I8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+      (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 };
 constexpr int NTHREADS = 192;                            // producer warp, MMA warp, four epilogue warps
-constexpr uint32_t WAIT_LIMIT = 1u << 20;
-constexpr int MAX_K8 = 131072;  // 127 * 127 * k stays below 2^31
 
 struct GemmArgs {
   const unsigned char* a;  // operand image of the rows: [m tile][2 K / 64][16 KB]
   const unsigned char* w;  // weight image: [n tile][K / 64][32 KB]
   const float* bias;       // (N) or null
   int M, N, K;
-  int mode;                // 0 operand image of the next product, 1 bf16 caches, 2 int8 caches, 3 4-bit caches, 4 rows
+  int mode;                // 0 operand image of the next product, 1 bf16 caches, 2 int8 caches, 3 4-bit caches
   int halves;              // of A: 2, or 1 when the rows are bf16 values (their low halves are zero, and not read)
   unsigned char* next;     // mode 0: [m tile][2 N / 64][16 KB]
   const int4* pieces;      // modes 1, 2: (n_pieces) {first row, frames, slot, 0}, first rows ascending from 0
@@ -66,94 +61,7 @@ struct GemmArgs {
   float* cvs;
   int S1, H, D, T;         // caches (layers, S1, H, T, D)
   int* status;
-  // 8-bit operands: images [m tile][K / 128][16 KB] and [n / 256][K / 128][32 KB], K rounded up to 128
-  const float* a_scale;    // (M)
-  const float* w_scale;    // (N)
-  void* out;               // mode 4: (M, ldo) of out_kind
-  int64_t ldo;
-  int out_kind, act;
 };
-
-DEVI uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-DEVI void mbar_init(uint64_t* bar, int count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-DEVI void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-DEVI void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-DEVI bool mbar_wait(uint64_t* bar, uint32_t parity) {  // bounded; false when the limit ran out
-  const uint32_t addr = smem_u32(bar);
-  for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
-}
-DEVI void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-DEVI void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-DEVI void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// K-major tile with the 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart
-DEVI uint64_t umma_desc(uint32_t saddr) {
-  uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-DEVI void umma_bf16(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-DEVI void umma_i8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-DEVI void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-// 64 consecutive columns of this warp's 32 tensor-memory lanes
-DEVI void tmem_ld64(uint32_t taddr, float (&v)[64]) {
-  uint32_t d[64];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t* e = d + 32 * h;
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(e[0]), "=r"(e[1]), "=r"(e[2]), "=r"(e[3]), "=r"(e[4]), "=r"(e[5]), "=r"(e[6]), "=r"(e[7]), "=r"(e[8]),
-          "=r"(e[9]), "=r"(e[10]), "=r"(e[11]), "=r"(e[12]), "=r"(e[13]), "=r"(e[14]), "=r"(e[15]), "=r"(e[16]),
-          "=r"(e[17]), "=r"(e[18]), "=r"(e[19]), "=r"(e[20]), "=r"(e[21]), "=r"(e[22]), "=r"(e[23]), "=r"(e[24]),
-          "=r"(e[25]), "=r"(e[26]), "=r"(e[27]), "=r"(e[28]), "=r"(e[29]), "=r"(e[30]), "=r"(e[31])
-        : "r"(taddr + 32 * h)
-        : "memory");
-  }
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(d[i]);
-}
-
-// byte offset of (row r, 16-byte chunk c) inside a K-major block of 128-byte rows with the 128-byte swizzle
-DEVI int swz(int r, int c) { return (r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4); }
 
 // v[0..63] + bias -> the two bf16 halves, as one 128-byte row each of the next product's operand image
 DEVI void store_operand_row(const float (&v)[64], unsigned char* hi_blk, unsigned char* lo_blk, int r) {
@@ -171,121 +79,16 @@ DEVI void store_operand_row(const float (&v)[64], unsigned char* hi_blk, unsigne
   }
 }
 
-// the reference's int8 cache format for 64 values already rounded to bf16, given the vector's absmax
-DEVI void store_q8_64(const float (&f)[64], float mx, int8_t* dst) {
-  const float sc = mx > 0.f ? __fdiv_rn(mx, 127.f) : 1.f, inv = __fdiv_rn(1.f, sc);
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int q = __float2int_rn(fminf(fmaxf(__fmul_rn(f[16 * c + i], inv), -127.f), 127.f));
-      w[i >> 2] |= (uint32_t)(q & 0xff) << ((i & 3) * 8);
-    }
-    *reinterpret_cast<uint4*>(dst + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
-// 64 values of a 4-bit group (kv4.cuh): the codes and the pair
-DEVI void store_q4_64(const float (&v)[64], uint8_t* codes, uint32_t* pair) {
-  float mn = INFINITY, mx = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < 64; ++i) {
-    const float x = kv4_clamp(__bfloat162float(__float2bfloat16_rn(v[i])));
-    mn = fminf(mn, x), mx = fmaxf(mx, x);
-  }
-  const Kv4Group g = kv4_group(mn, mx);
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      w[i >> 3] |= (uint32_t)kv4_code(kv4_clamp(__bfloat162float(__float2bfloat16_rn(v[32 * c + i]))), g) << ((i & 7) * 4);
-    *reinterpret_cast<uint4*>(codes + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  *pair = g.word;
-}
-
-DEVI float activate(float x, int act) {
-  if (act == B200DEC_ACT_RELU) return fmaxf(x, 0.f);
-  if (act == B200DEC_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-  return x;
-}
-
-// 32-bit sums of a row's columns n0 .. n0 + 63 -> (sum * (row scale * channel scale)) + bias; columns past N are left as they are
-DEVI void scale_row(const GemmArgs& p, float (&v)[64], int n0, float sa) {
-  const bool whole = n0 + 64 <= p.N;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float w[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (whole) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(p.w_scale + n0) + i);
-      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-      if (p.bias) {
-        const float4 y = __ldg(reinterpret_cast<const float4*>(p.bias + n0) + i);
-        b[0] = y.x, b[1] = y.y, b[2] = y.z, b[3] = y.w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n0 + 4 * i + j < p.N) w[j] = __ldg(p.w_scale + n0 + 4 * i + j), b[j] = p.bias ? __ldg(p.bias + n0 + 4 * i + j) : 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float& x = v[4 * i + j];
-      x = __fadd_rn(__fmul_rn(__int2float_rn(__float_as_int(x)), __fmul_rn(sa, w[j])), b[j]);
-    }
-  }
-  if (p.act != B200DEC_ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < 64; ++i) v[i] = activate(v[i], p.act);
-  }
-}
-
-// 64 result values of a row, columns n0 .. n0 + 63 of which those below N are stored
-template <class T>
-DEVI T out_value(float x) {
-  if constexpr (sizeof(T) == 4) return x;
-  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
-  else return __float2bfloat16_rn(x);
-}
-template <class T>
-DEVI void store_row_64(const float (&v)[64], T* dst, int n, bool wide) {
-  if (wide && n >= 64) {  // 32 bytes at a time: whole sectors
-    constexpr int PER = 32 / (int)sizeof(T);
-#pragma unroll
-    for (int c = 0; c < 64 / PER; ++c) {
-      uint32_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[c * PER + i]);
-        else {
-          const T a = out_value<T>(v[c * PER + 2 * i]), b = out_value<T>(v[c * PER + 2 * i + 1]);
-          w[i] = (uint32_t)reinterpret_cast<const unsigned short&>(a) | ((uint32_t)reinterpret_cast<const unsigned short&>(b) << 16);
-        }
-      }
-      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c * PER), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                   "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                   : "memory");
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 64; ++i)
-      if (i < n) dst[i] = out_value<T>(v[i]);
-  }
-}
-
-template <int TN, bool I8>
+template <int TN>
 __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArgs p) {
-  using Cfg = Tile<TN, I8>;
-  constexpr int STAGES = Cfg::STAGES, B_STAGE = Cfg::B_STAGE, STAGE_BYTES = Cfg::STAGE_BYTES;
+  constexpr int STAGES = Tile<TN>::STAGES, B_STAGE = Tile<TN>::B_STAGE, STAGE_BYTES = Tile<TN>::STAGE_BYTES;
   extern __shared__ unsigned char dyn_smem[];
   unsigned char* smem = dyn_smem + ((1024 - (smem_u32(dyn_smem) & 1023)) & 1023);
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2];
   __shared__ uint32_t tmem_base;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int MT = (p.M + BM - 1) / BM, NT = (p.N + TN - 1) / TN, NKB = p.K / (I8 ? 2 * BK : BK);
+  const int MT = (p.M + BM - 1) / BM, NT = p.N / TN, NKB = p.K / BK;
   const int tiles = MT * NT;
 
   if (tid == 0) {
@@ -298,7 +101,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArg
   pdl_wait();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
-                 "n"(Cfg::TMEM_COLS)
+                 "n"(Tile<TN>::TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -320,12 +123,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArg
           ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1);
           if (!ok) break;
           unsigned char* st = smem + s * STAGE_BYTES;
-          mbar_expect_tx(&full[s], (I8 ? 1 : p.halves) * A_STAGE + B_STAGE);
-          const unsigned char* a = p.a + ((size_t)mt * (I8 ? 1 : 2) * NKB + kb) * A_STAGE;
+          mbar_expect_tx(&full[s], p.halves * A_STAGE + B_STAGE);
+          const unsigned char* a = p.a + ((size_t)mt * 2 * NKB + kb) * A_STAGE;
           bulk_load(st, a, A_STAGE, &full[s]);
-          if (!I8 && p.halves > 1) bulk_load(st + A_STAGE, a + (size_t)NKB * A_STAGE, A_STAGE, &full[s]);
+          if (p.halves > 1) bulk_load(st + A_STAGE, a + (size_t)NKB * A_STAGE, A_STAGE, &full[s]);
           const int n0 = nt * TN;
-          bulk_load(st + Cfg::A_BYTES, p.w + ((size_t)(n0 / BN) * NKB + kb) * B_BLOCK + n0 % BN / TN * B_STAGE, B_STAGE, &full[s]);
+          bulk_load(st + 2 * A_STAGE, p.w + ((size_t)(n0 / BN) * NKB + kb) * B_BLOCK + n0 % BN / TN * B_STAGE, B_STAGE, &full[s]);
         }
       }
       if (!ok) {
@@ -354,18 +157,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArg
           ok = mbar_wait(&full[s], (it / STAGES) & 1);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + s * STAGE_BYTES), b0 = a0 + Cfg::A_BYTES;
-          if constexpr (I8) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)  // 32 k each
-              umma_i8(acc, umma_desc(a0 + k * 32), umma_desc(b0 + k * 32), Cfg::IDESC, (kb | k) != 0);
-          } else {
+          const uint32_t a0 = smem_u32(smem + s * STAGE_BYTES), b0 = a0 + 2 * A_STAGE;
 #pragma unroll 1
-            for (int h = 0; h < p.halves; ++h)
+          for (int h = 0; h < p.halves; ++h)
 #pragma unroll
-              for (int k = 0; k < BK / 16; ++k)
-                umma_bf16(acc, umma_desc(a0 + h * A_STAGE + k * 32), umma_desc(b0 + k * 32), Cfg::IDESC, (kb | h | k) != 0);
-          }
+            for (int k = 0; k < BK / 16; ++k)
+              umma_bf16(acc, umma_desc(a0 + h * A_STAGE + k * 32), umma_desc(b0 + k * 32), Tile<TN>::IDESC, (kb | h | k) != 0);
           umma_commit(&empty[s]);  // the stage is free once these MMAs have read it
         }
         if (ok) umma_commit(&tfull[buf]);
@@ -386,8 +183,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArg
       const uint32_t acc = tmem_d + buf * TN + ((uint32_t)(q * 32) << 16);
       const int m = mt * BM + row;
       int slot = -1, frame = 0;
-      const float sa = I8 && m < p.M ? __ldg(p.a_scale + m) : 0.f;
-      if (p.mode != 0 && p.mode != 4 && m < p.M) {  // the piece that holds row m: the last one that starts at or before it
+      if (p.mode != 0 && m < p.M) {  // the piece that holds row m: the last one that starts at or before it
         int lo = 0, hi = p.n_pieces - 1;
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
@@ -402,31 +198,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArg
         const int n0 = nt * TN + c0;
         float v[64];
         tmem_ld64(acc + c0, v);
-        if constexpr (I8) scale_row(p, v, n0, sa);
-        else if (p.bias) {
+        if (p.bias) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + n0) + i);
             v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
-          }
-        }
-        if constexpr (I8) {
-          if (p.mode == 4) {
-            if (m < p.M && n0 < p.N) {
-              const size_t at = (size_t)m * p.ldo + n0;
-              const int n = p.N - n0;
-              if (p.out_kind == B200DEC_T_F32) {
-                float* d = reinterpret_cast<float*>(p.out) + at;
-                store_row_64(v, d, n, ((uintptr_t)d & 31) == 0);
-              } else if (p.out_kind == B200DEC_T_F16) {
-                __half* d = reinterpret_cast<__half*>(p.out) + at;
-                store_row_64(v, d, n, ((uintptr_t)d & 31) == 0);
-              } else {
-                __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(p.out) + at;
-                store_row_64(v, d, n, ((uintptr_t)d & 31) == 0);
-              }
-            }
-            continue;
           }
         }
         if (p.mode == 0) {
@@ -468,10 +244,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArg
             // D = 128: this chunk is the first half of its vector (c0 % 128 == 0); fetch the second, then both go out
             float u[64];
             tmem_ld64(acc + c0 + 64, u);
-            if constexpr (I8) scale_row(p, u, n0 + 64, sa);
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
-              const float b = !I8 && p.bias ? __ldg(p.bias + n0 + 64 + i) : 0.f;
+              const float b = p.bias ? __ldg(p.bias + n0 + 64 + i) : 0.f;
               u[i] = __bfloat162float(__float2bfloat16_rn(u[i] + b));
               mx = fmaxf(mx, fabsf(u[i]));
             }
@@ -495,7 +270,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArg
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "n"(Cfg::TMEM_COLS) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "n"(Tile<TN>::TMEM_COLS) : "memory");
   }
 }
 
@@ -532,120 +307,15 @@ __global__ void pack_rows_kernel(const X* __restrict__ x, int m, int k, int ldx,
     *reinterpret_cast<uint4*>(tile + (size_t)(nkb + kb) * A_STAGE + swz(r % BM, chunk)) = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// ---- 8-bit operands --------------------------------------------------------------------------------------------------------
-// Rows -> 8-bit integers with one scale a row: s = max(max |x|, 1e-12) / 127, q = rint(x / s), both as if the quotients were
-// exact: the product with the reciprocal is off by a few 2^-23 of it, so only its rounding beside a half can be wrong, and
-// the remainder x - q s (exact: a multiple of ulp(s) / 2 below 2^24 of them) decides there. A row with an infinity or NaN gets
-// scale NaN: its results are NaN. One warp a row, which passes over it twice (the second time out of L1 and L2).
-template <class X>
-DEVI float row_value(X x) {
-  if constexpr (std::is_same<X, float>::value) return x;
-  else if constexpr (std::is_same<X, __half>::value) return __half2float(x);
-  else return __bfloat162float(x);
-}
-
-// values c .. c + 15 of a row of k, zeros past its end
-template <class X, bool WIDE>
-DEVI void load_16(const X* row, int c, int k, float (&f)[16]) {
-  if (WIDE && c + 16 <= k) {
-    constexpr int PER = 16 / (int)sizeof(X);
-#pragma unroll
-    for (int i = 0; i < 16 / PER; ++i) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
-      X x[PER];
-      memcpy(x, &w, 16);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) f[i * PER + j] = row_value(x[j]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = c + i < k ? row_value(row[c + i]) : 0.f;
-  }
-}
-
-DEVI int code8(float x, float s, float inv) {
-  float c = fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
-  const float e2 = 2.f * __fmaf_rn(-c, s, x);
-  const bool odd = ((int)c & 1) != 0;
-  if (e2 > s || (e2 == s && odd)) c += 1.f;
-  if (-e2 > s || (-e2 == s && odd)) c -= 1.f;
-  return (int)fminf(fmaxf(c, -127.f), 127.f);
-}
-
-template <class X, bool WIDE>
-__global__ void __launch_bounds__(256) pack_rows_i8_kernel(const X* __restrict__ x, int m, int k, int64_t ldx,
-                                                           unsigned char* __restrict__ image, float* __restrict__ scale) {
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  pdl_wait();
-  pdl_trigger();
-  if (row >= m) return;  // the rows that fill the last tile up are never stored: whatever the image holds there does no harm
-  const X* src = x + row * ldx;
-  uint32_t top = 0;  // largest magnitude by its bits, so that a NaN is the largest
-  for (int c = lane * 16; c < k; c += 512) {
-    float f[16];
-    load_16<X, WIDE>(src, c, k, f);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  const float s = top < 0x7f800000u ? __fdiv_rn(fmaxf(__uint_as_float(top), 1e-12f), 127.f) : __uint_as_float(0x7fffffffu);
-  const float inv = __frcp_rn(s);
-  if (lane == 0) scale[row] = s;
-  const int kp = (k + 127) / 128 * 128;
-  unsigned char* tile = image + (size_t)(row / BM) * (kp / 128) * A_STAGE;
-  for (int c = lane * 16; c < kp; c += 512) {
-    float f[16];
-    load_16<X, WIDE>(src, c, k, f);
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i >> 2] |= (uint32_t)(code8(f[i], s, inv) & 0xff) << ((i & 3) * 8);
-    *reinterpret_cast<uint4*>(tile + (size_t)(c / 128) * A_STAGE + swz(row % BM, (c % 128) / 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
-// int8 weights (n, k) row-major -> [n / 256][k / 128][256 rows x 128 B, swizzled], zeros where n or k end; a thread per 16 bytes
-__global__ void tile_weight_i8_kernel(const int8_t* __restrict__ q, int n, int k, unsigned char* __restrict__ out) {
-  const int np = (n + BN - 1) / BN * BN, kp = (k + 127) / 128 * 128, cpr = kp / 16;
-  const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (size_t)np * cpr) return;
-  const int r = (int)(i / cpr), c = (int)(i % cpr);
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (r < n && c * 16 + j < k) w[j >> 2] |= (uint32_t)(uint8_t)q[(size_t)r * k + c * 16 + j] << ((j & 3) * 8);
-  *reinterpret_cast<uint4*>(out + ((size_t)(r / BN) * (kp / 128) + c / 8) * B_BLOCK + swz(r % BN, c % 8)) =
-      make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-template <class X>
-cudaError_t launch_pack_i8(const void* x, int m, int k, int64_t ldx, void* image, float* scale, cudaStream_t st) {
-  const bool wide = ((uintptr_t)x & 15) == 0 && (m == 1 || ldx * sizeof(X) % 16 == 0);
-  const dim3 grid((m + 7) / 8);
-  if (wide) pack_rows_i8_kernel<X, true><<<grid, 256, 0, st>>>((const X*)x, m, k, ldx, (unsigned char*)image, scale);
-  else pack_rows_i8_kernel<X, false><<<grid, 256, 0, st>>>((const X*)x, m, k, ldx, (unsigned char*)image, scale);
-  return cudaGetLastError();
-}
-
-template <int TN, bool I8>
+template <int TN>
 int launch_gemm(const GemmArgs& a, int sms, cudaStream_t stream) {
-  constexpr int BYTES = Tile<TN, I8>::SMEM_BYTES;
-  cudaError_t e = cudaFuncSetAttribute(prefill_gemm_kernel<TN, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+  constexpr int BYTES = Tile<TN>::SMEM_BYTES;
+  cudaError_t e = cudaFuncSetAttribute(prefill_gemm_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
   if (e != cudaSuccess) return fail(B200DEC_ECUDA, "prefill_gemm: smem attribute: %s", cudaGetErrorString(e));
-  const int tiles = ((a.M + BM - 1) / BM) * ((a.N + TN - 1) / TN);
-  e = launch_kernel(prefill_gemm_kernel<TN, I8>, dim3(tiles < sms ? tiles : sms), dim3(NTHREADS), BYTES, stream, 0, true, a);
+  const int tiles = ((a.M + BM - 1) / BM) * (a.N / TN);
+  e = launch_kernel(prefill_gemm_kernel<TN>, dim3(tiles < sms ? tiles : sms), dim3(NTHREADS), BYTES, stream, 0, true, a);
   if (e != cudaSuccess) return fail(B200DEC_ECUDA, "prefill_gemm launch: %s", cudaGetErrorString(e));
   return 0;
-}
-
-// The widest tile that leaves no SM idle; narrower ones as long as the tiles still are one wave.
-int launch_i8(const GemmArgs& a, cudaStream_t stream) {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t mt = (a.M + BM - 1) / BM;
-  B200_REQUIRE(mt * ((a.N + 63) / 64) < 1 << 30, "w8a8: m %d x n %d", a.M, a.N);
-  if (a.mode == 4 && mt * ((a.N + 63) / 64) <= sms) return launch_gemm<64, true>(a, sms, stream);
-  if (a.mode == 4 && mt * ((a.N + 127) / 128) <= sms) return launch_gemm<128, true>(a, sms, stream);
-  return launch_gemm<BN, true>(a, sms, stream);
 }
 
 // bf16 weights (n, k) row-major -> the weight image [n / 256][k / 64][256 rows x 128 B, swizzled]; one thread per 16 B
@@ -725,79 +395,8 @@ int b200dec_prefill_gemm(const void* rows_image, int m, int k, const void* weigh
   // the rows would be copied again by every further wave. Both products, us on the device with narrow / wide tiles in the first:
   // 30.6 / 35.8 at 175 frames, 53.0 / 57.2 at 640, 67.0 / 72.0 at 1152 (one wave of 144). With the products launched behind
   // one another programmatically and bf16 rows packed as they are, a prefill of 175 bf16 frames went from 40.6 to 28.1.
-  if (mode == 0 && ((m + BM - 1) / BM) * (n / 64) <= sms) return launch_gemm<64, false>(a, sms, (cudaStream_t)stream);
-  return launch_gemm<BN, false>(a, sms, (cudaStream_t)stream);
-}
-
-int64_t b200dec_w8a8_rows_bytes(int m, int k) {
-  if (m < 0 || k <= 0 || k > MAX_K8) return -1;
-  return (int64_t)((m + BM - 1) / BM) * BM * ((k + 127) / 128 * 128);
-}
-
-int64_t b200dec_w8a8_weight_bytes(int n, int k) {
-  if (n <= 0 || k <= 0 || k > MAX_K8) return -1;
-  return (int64_t)((n + BN - 1) / BN) * BN * ((k + 127) / 128 * 128);
-}
-
-int b200dec_w8a8_pack_rows(const void* x, int kind, int m, int k, int64_t ldx, void* image, float* scale, void* stream) {
-  B200_REQUIRE(x && image && scale, "w8a8_pack_rows: null pointer");
-  B200_REQUIRE(m >= 1 && k >= 1 && k <= MAX_K8 && (m == 1 || ldx >= k), "w8a8_pack_rows: m %d k %d ldx %lld", m, k, (long long)ldx);
-  B200_REQUIRE(kind == B200DEC_T_F32 || kind == B200DEC_T_F16 || kind == B200DEC_T_BF16, "w8a8_pack_rows: kind %d", kind);
-  B200_REQUIRE(((uintptr_t)image & 1023) == 0 && (uintptr_t)x % (kind == B200DEC_T_F32 ? 4 : 2) == 0,
-               "w8a8_pack_rows: alignment (the image 1 KB)");
-  const cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = kind == B200DEC_T_F32   ? launch_pack_i8<float>(x, m, k, ldx, image, scale, st)
-                        : kind == B200DEC_T_F16 ? launch_pack_i8<__half>(x, m, k, ldx, image, scale, st)
-                                                : launch_pack_i8<__nv_bfloat16>(x, m, k, ldx, image, scale, st);
-  if (e != cudaSuccess) return fail(B200DEC_ECUDA, "w8a8_pack_rows launch: %s", cudaGetErrorString(e));
-  return 0;
-}
-
-int b200dec_w8a8_tile_weight(const int8_t* q, int n, int k, void* image, void* stream) {
-  B200_REQUIRE(q && image && n >= 1 && k >= 1 && k <= MAX_K8 && ((uintptr_t)image & 1023) == 0,
-               "w8a8_tile_weight: (%d, %d) into a 1 KB aligned image", n, k);
-  const size_t total = (size_t)b200dec_w8a8_weight_bytes(n, k) / 16;
-  tile_weight_i8_kernel<<<(unsigned)((total + 255) / 256), 256, 0, (cudaStream_t)stream>>>(q, n, k, (unsigned char*)image);
-  return check_launch("w8a8_tile_weight");
-}
-
-int b200dec_w8a8_linear(const void* rows_image, const float* row_scale, int m, int k, const void* weight_image,
-                        const float* w_scale, const float* bias, int n, int act, void* out, int out_kind, int64_t ldo,
-                        int32_t* status, void* stream) {
-  B200_REQUIRE(rows_image && row_scale && weight_image && w_scale && out && status, "w8a8_linear: null pointer");
-  B200_REQUIRE(m >= 1 && n >= 1 && k >= 1 && k <= MAX_K8 && (m == 1 || ldo >= n), "w8a8_linear: m %d k %d n %d ldo %lld", m, k, n,
-               (long long)ldo);
-  B200_REQUIRE(out_kind == B200DEC_T_F32 || out_kind == B200DEC_T_F16 || out_kind == B200DEC_T_BF16, "w8a8_linear: out_kind %d", out_kind);
-  B200_REQUIRE(act == B200DEC_ACT_NONE || act == B200DEC_ACT_RELU || act == B200DEC_ACT_GELU, "w8a8_linear: act %d", act);
-  B200_REQUIRE((((uintptr_t)rows_image | (uintptr_t)weight_image) & 1023) == 0 && (((uintptr_t)w_scale | (uintptr_t)bias) & 15) == 0 &&
-                   (uintptr_t)out % (out_kind == B200DEC_T_F32 ? 4 : 2) == 0,
-               "w8a8_linear: alignment (images 1 KB, channel scales and bias 16 bytes)");
-  GemmArgs a{};
-  a.a = (const unsigned char*)rows_image, a.w = (const unsigned char*)weight_image, a.bias = bias;
-  a.M = m, a.N = n, a.K = (k + 127) / 128 * 128, a.mode = 4, a.status = status;
-  a.a_scale = row_scale, a.w_scale = w_scale, a.out = out, a.ldo = ldo, a.out_kind = out_kind, a.act = act;
-  return launch_i8(a, (cudaStream_t)stream);
-}
-
-int b200dec_w8a8_prefill(const void* rows_image, const float* row_scale, int m, int k, const void* weight_image,
-                         const float* w_scale, const float* bias, int n, int mode, const int32_t* pieces, int n_pieces, void* ck,
-                         void* cv, void* ck_scale, void* cv_scale, int layers, int slots_plus_1, int heads, int head_dim, int frames,
-                         int32_t* status, void* stream) {
-  B200_REQUIRE(rows_image && row_scale && weight_image && w_scale && status, "w8a8_prefill: null pointer");
-  B200_REQUIRE(m >= 1 && k >= 1 && k <= MAX_K8 && mode >= 1 && mode <= 3, "w8a8_prefill: m %d k %d mode %d", m, k, mode);
-  B200_REQUIRE(pieces && n_pieces >= 1 && ck && cv && (mode == 1 || (ck_scale && cv_scale)), "w8a8_prefill: pieces and caches");
-  B200_REQUIRE((((uintptr_t)rows_image | (uintptr_t)weight_image) & 1023) == 0 &&
-                   (((uintptr_t)w_scale | (uintptr_t)bias | (uintptr_t)pieces | (uintptr_t)ck | (uintptr_t)cv) & 15) == 0,
-               "w8a8_prefill: alignment (images 1 KB, the rest 16 bytes)");
-  B200_REQUIRE((head_dim == 64 || head_dim == 128) && layers >= 1 && heads >= 1 && slots_plus_1 >= 1 && frames >= 1 &&
-                   (int64_t)n == (int64_t)layers * 2 * heads * head_dim && n % BN == 0,
-               "w8a8_prefill: n %d != layers %d x 2 x heads %d x head_dim %d (a multiple of 256)", n, layers, heads, head_dim);
-  GemmArgs a{};
-  a.a = (const unsigned char*)rows_image, a.w = (const unsigned char*)weight_image, a.bias = bias;
-  a.M = m, a.N = n, a.K = (k + 127) / 128 * 128, a.mode = mode, a.status = status, a.a_scale = row_scale, a.w_scale = w_scale;
-  a.pieces = (const int4*)pieces, a.n_pieces = n_pieces, a.ck = ck, a.cv = cv, a.cks = (float*)ck_scale, a.cvs = (float*)cv_scale;
-  a.S1 = slots_plus_1, a.H = heads, a.D = head_dim, a.T = frames;
-  return launch_i8(a, (cudaStream_t)stream);
+  if (mode == 0 && ((m + BM - 1) / BM) * (n / 64) <= sms) return launch_gemm<64>(a, sms, (cudaStream_t)stream);
+  return launch_gemm<BN>(a, sms, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,566 @@
+// A product of 8-bit integers on the fifth-generation tensor cores: y = act((q_x q_w^T) * s_x * s_w + bias), q_x quantised per row as
+// the rows come, q_w and s_w per channel at init time. The result goes to fp32, fp16 or bf16 rows, or straight into the slot
+// caches (the cross-attention prefill in 8 bits).
+//
+// Both operands lie in global memory as the images of their shared-memory tiles (rows of 128 bytes = 128 k, 128-byte swizzle), so a
+// pipeline stage is two plain cp.async.bulk copies. tcgen05.mma kind::i8 multiplies M 128 x N TN x K 32 into 32-bit integer
+// accumulators in tensor memory: the sums are exact, and every later operation rounds once.
+//   * persistent CTAs walk the (channel tile, row tile) list: warp 0 feeds the ring, warp 1 issues the MMAs into one of two
+//     accumulators, warps 2-9 drain the other: two warps per 32 lanes, each half of the tile's columns. Per k the MMA is twice as
+//     fast as with 16-bit operands, so the epilogue, not the operands, decides unless eight warps share it: a tile of 128 x 256 x
+//     1024 multiplies for about 4 100 cycles, and four warps took 24 000 to scale, round and store it.
+//   * channel scales and biases of a tile go to shared memory once, as pairs, and are read back as broadcasts.
+//   * rows leave in whole 32-byte sectors, a thread per row; rows that are not 32-byte aligned through a transposition in shared
+//     memory, so that a warp's store still covers whole lines.
+// Every mbarrier wait is bounded; a wait that runs out sets B200DEC_ST_TIMEOUT, the roles fall through, copies in flight are
+// awaited (bounded) and tensor memory is released.
+#include <type_traits>
+
+#include "kv_store.cuh"
+#include "umma.cuh"
+
+using namespace b200dec_detail;
+
+namespace {
+
+constexpr int BM = UMMA_BM, BN = UMMA_BN, MAX_K8 = 131072;  // 127 * 127 * k stays below 2^31
+constexpr int EPI_WARPS = 8, NTHREADS = 64 + 32 * EPI_WARPS, TR_COLS = 16, TR_LD = TR_COLS + 1;
+
+template <int TN>
+struct Tile {
+  static constexpr int B_STAGE = TN * 128, STAGE_BYTES = A_STAGE + B_STAGE, STAGES = TN == 256 ? 4 : TN == 128 ? 6 : 8;
+  static constexpr int PAIRS = STAGES * STAGE_BYTES, TR = PAIRS + 2 * TN * 8;  // {scale, bias} per column and accumulator
+  static constexpr int SMEM_BYTES = TR + EPI_WARPS * 32 * TR_LD * 4 + 1024;     // slack to align the base to a swizzle atom
+  static constexpr int TMEM_COLS = 2 * TN;
+  // signed 8-bit x signed 8-bit -> 32-bit, both operands K-major, M = 128, N = TN
+  static constexpr uint32_t IDESC =
+      (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+};
+
+struct W8Args {
+  const unsigned char* a;  // rows: [m tile][K / 128][16 KB]
+  const unsigned char* w;  // weights: [n / 256][K / 128][32 KB]
+  const float* a_scale;    // (M)
+  const float* w_scale;    // (N)
+  const float* bias;       // (N) or null
+  int M, N, NKB;           // NKB: blocks of 128 k
+  int mode;                // 1 bf16 caches, 2 int8 caches, 3 4-bit caches, 4 rows
+  int act;
+  void* out;               // mode 4: (M, ldo) of out_kind
+  int64_t ldo;
+  int out_kind;
+  const int4* pieces;      // modes 1-3: (n_pieces) {first row, frames, slot, 0}, first rows ascending from 0
+  int n_pieces;
+  void* ck;
+  void* cv;
+  float* cks;
+  float* cvs;
+  int S1, H, D, T;         // caches (layers, S1, H, T, D)
+  int* status;
+};
+
+DEVI void umma_i8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+DEVI void epi_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory"); }
+
+DEVI float activate(float x, int act) {
+  if (act == B200DEC_ACT_RELU) return fmaxf(x, 0.f);
+  if (act == B200DEC_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+  return x;
+}
+
+// 32 sums of a row -> values: (sum * (row scale * channel scale)) + bias, pr: the columns' {scale, bias}
+DEVI void finish32(const uint32_t (&e)[32], float* v, const float2* pr, float sa, int act) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const float4 p = *reinterpret_cast<const float4*>(pr + i);
+    v[i] = __fadd_rn(__fmul_rn(__int2float_rn((int)e[i]), __fmul_rn(sa, p.x)), p.y);
+    v[i + 1] = __fadd_rn(__fmul_rn(__int2float_rn((int)e[i + 1]), __fmul_rn(sa, p.z)), p.w);
+  }
+  if (act != B200DEC_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = activate(v[i], act);
+  }
+}
+
+template <class T>
+DEVI T out_value(float x) {
+  if constexpr (std::is_same<T, float>::value) return x;
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
+  else return __float2bfloat16_rn(x);
+}
+DEVI uint32_t pair_of(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return reinterpret_cast<const uint32_t&>(h);
+}
+DEVI uint32_t pair_of(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
+DEVI void st_sector(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// 32 columns of the warp's 32 rows (a row per thread) from row m0 on, column n0 on, into T rows
+template <class T>
+DEVI void store_rows(const W8Args& p, const float* v, int m0, int n0, int lane, bool wide, float* tr) {
+  T* out = reinterpret_cast<T*>(p.out);
+  if (wide && n0 + 32 <= p.N) {
+    if (m0 + lane < p.M) {
+      T* d = out + (size_t)(m0 + lane) * p.ldo + n0;
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * c + i]);
+          st_sector(d + 8 * c, w);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = pair_of(v[16 * c + 2 * i], v[16 * c + 2 * i + 1], T());
+          st_sector(d + 16 * c, w);
+        }
+      }
+    }
+    return;
+  }
+  // 16 columns at a time through shared memory: a store instruction then covers two rows' runs of 16 columns
+#pragma unroll
+  for (int c = 0; c < 32; c += TR_COLS) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < TR_COLS; ++i) tr[lane * TR_LD + i] = v[c + i];
+    __syncwarp();
+    const int col = n0 + c + (lane & 15);
+    if (col < p.N) {
+#pragma unroll 4
+      for (int r = lane >> 4; r < 32; r += 2)
+        if (m0 + r < p.M) out[(size_t)(m0 + r) * p.ldo + col] = out_value<T>(tr[r * TR_LD + (lane & 15)]);
+    }
+  }
+}
+
+template <int TN>
+__global__ void __launch_bounds__(NTHREADS, 1) w8a8_kernel(const W8Args p) {
+  using Cfg = Tile<TN>;
+  constexpr int STAGES = Cfg::STAGES, STAGE_BYTES = Cfg::STAGE_BYTES, B_STAGE = Cfg::B_STAGE;
+  extern __shared__ unsigned char dyn_smem[];
+  unsigned char* smem = dyn_smem + ((1024 - (smem_u32(dyn_smem) & 1023)) & 1023);
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2];
+  __shared__ uint32_t tmem_base;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int MT = (p.M + BM - 1) / BM, NT = (p.N + TN - 1) / TN, NKB = p.NKB;
+  const int64_t tiles = (int64_t)MT * NT;
+  const auto weights = [&](int nt, int kb) {
+    const int n0 = nt * TN;
+    return p.w + ((size_t)(n0 / BN) * NKB + kb) * B_BLOCK + n0 % BN / TN * B_STAGE;
+  };
+
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&tfull[i], 1), mbar_init(&tempty[i], EPI_WARPS);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // the first tile's weights are nobody's output: on their way before the wait for the kernel that quantises the rows
+    for (int kb = 0; kb < min(NKB, STAGES); ++kb) {
+      mbar_expect_tx(&full[kb], STAGE_BYTES);
+      bulk_load(smem + kb * STAGE_BYTES + A_STAGE, weights(blockIdx.x / MT, kb), B_STAGE, &full[kb]);
+    }
+  }
+  pdl_wait();  // ahead of the allocation, so that no CTA sits on tensor memory while it waits
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                 "n"(Cfg::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_d = tmem_base;
+  pdl_trigger();
+
+  if (warp == 0) {
+    // ---- producer: two bulk copies per stage ----------------------------------------------------------------------------
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t it = 0;
+      for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+        const int mt = (int)(tile % MT), nt = (int)(tile / MT);
+        for (int kb = 0; kb < NKB; ++kb, ++it) {
+          const int s = it % STAGES;
+          unsigned char* st = smem + s * STAGE_BYTES;
+          if (it >= (uint32_t)min(NKB, STAGES)) {
+            ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1);
+            if (!ok) break;
+            mbar_expect_tx(&full[s], STAGE_BYTES);
+            bulk_load(st + A_STAGE, weights(nt, kb), B_STAGE, &full[s]);
+          }
+          bulk_load(st, p.a + ((size_t)mt * NKB + kb) * A_STAGE, A_STAGE, &full[s]);
+        }
+      }
+      if (!ok) {
+        atomicOr(p.status, B200DEC_ST_TIMEOUT);
+        // the copies already issued must land before this CTA's shared memory is given away
+        const uint32_t issued = it < (uint32_t)STAGES ? it : (uint32_t)STAGES;
+        for (uint32_t i = 0; i < issued; ++i) {
+          const uint32_t jt = it - 1 - i;
+          mbar_wait(&full[jt % STAGES], (jt / STAGES) & 1);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMA issue: one lane --------------------------------------------------------------------------------------------
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t it = 0, tc = 0;
+      for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++tc) {
+        const uint32_t buf = tc & 1;
+        ok = mbar_wait(&tempty[buf], ((tc >> 1) & 1) ^ 1);  // the epilogue has drained this accumulator
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = tmem_d + buf * TN;
+        for (int kb = 0; kb < NKB; ++kb, ++it) {
+          const int s = it % STAGES;
+          ok = mbar_wait(&full[s], (it / STAGES) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(smem + s * STAGE_BYTES), b0 = a0 + A_STAGE;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // 32 k = 32 bytes each
+            umma_i8(acc, umma_desc(a0 + k * 32), umma_desc(b0 + k * 32), Cfg::IDESC, (kb | k) != 0);
+          umma_commit(&empty[s]);  // the stage is free once these MMAs have read it
+        }
+        if (ok) umma_commit(&tfull[buf]);
+      }
+      if (!ok) atomicOr(p.status, B200DEC_ST_TIMEOUT);
+    }
+  } else {
+    // ---- epilogue: warp w reads tensor-memory lanes 32 (w % 4) .. + 31, the first four the low half of the columns ----------
+    const int q = warp & 3, row = q * 32 + lane, half = (warp - 2) >> 2, et = tid - 64;
+    constexpr int HALF = TN / 2;
+    float* tr = reinterpret_cast<float*>(smem + Cfg::TR) + (warp - 2) * 32 * TR_LD;
+    const int size = p.out_kind == B200DEC_T_F32 ? 4 : 2;
+    const bool wide = ((uintptr_t)p.out & 31) == 0 && p.ldo * size % 32 == 0;
+    bool ok = true;
+    uint32_t tc = 0;
+    // what a tile needs from global memory is fetched a tile ahead: this thread's column's {scale, bias}, its row's scale
+    static_assert(TN <= 32 * EPI_WARPS, "one column per epilogue thread");
+    float2 pair_next;
+    float sa_next;
+    const auto fetch = [&](int64_t tile) {
+      const int m = (int)(tile % MT) * BM + row, n = (int)(tile / MT) * TN + et;
+      const bool has = tile < tiles && et < TN && n < p.N;
+      pair_next = make_float2(has ? __ldg(p.w_scale + n) : 0.f, has && p.bias ? __ldg(p.bias + n) : 0.f);
+      sa_next = tile < tiles && m < p.M ? __ldg(p.a_scale + m) : 0.f;
+    };
+    fetch(blockIdx.x);
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++tc) {  // after a time-out too: all meet at the barriers
+      const int mt = (int)(tile % MT), nt = (int)(tile / MT), buf = tc & 1;
+      const int m = mt * BM + row;
+      // the pairs go into the buffer of two tiles ago, which every warp has left (it passed the barrier of the tile between)
+      float2* pairs = reinterpret_cast<float2*>(smem + Cfg::PAIRS) + buf * TN;
+      if (et < TN) pairs[et] = pair_next;
+      const float sa = sa_next;
+      fetch(tile + gridDim.x);
+      int slot = -1, frame = 0;
+      if (p.mode != 4 && m < p.M) {  // the piece that holds row m: the last one that starts at or before it
+        int lo = 0, hi = p.n_pieces - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (__ldg(&p.pieces[mid].x) <= m) lo = mid;
+          else hi = mid - 1;
+        }
+        const int4 pc = __ldg(&p.pieces[lo]);
+        frame = m - pc.x;
+        if (frame >= 0 && frame < pc.y && frame < p.T && pc.z >= 0 && pc.z < p.S1) slot = pc.z;
+      }
+      epi_barrier();
+      if (ok) ok = mbar_wait(&tfull[buf], (tc >> 1) & 1);
+      if (!ok) continue;
+      tc_fence_after();
+      const uint32_t acc = tmem_d + buf * TN + half * HALF + ((uint32_t)(q * 32) << 16);
+      const float2* pr = pairs + half * HALF;
+      const int n0 = nt * TN + half * HALF;
+      if (p.mode == 4) {
+        uint32_t e[2][32];
+        tmem_ld32(acc, e[0]);
+#pragma unroll
+        for (int c = 0; c < HALF / 32; ++c) {
+          tmem_wait();
+          if (c + 1 < HALF / 32) tmem_ld32(acc + 32 * (c + 1), e[(c + 1) & 1]);
+          if (n0 + 32 * c >= p.N) continue;
+          float v[32];
+          finish32(e[c & 1], v, pr + 32 * c, sa, p.act);
+          if (p.out_kind == B200DEC_T_F32) store_rows<float>(p, v, mt * BM + q * 32, n0 + 32 * c, lane, wide, tr);
+          else if (p.out_kind == B200DEC_T_F16) store_rows<__half>(p, v, mt * BM + q * 32, n0 + 32 * c, lane, wide, tr);
+          else store_rows<__nv_bfloat16>(p, v, mt * BM + q * 32, n0 + 32 * c, lane, wide, tr);
+        }
+      } else if constexpr (TN == BN) {
+        // caches: 64 channels at a time; channel n = ((layer * 2 + k|v) * H + head) * D + d
+        const auto load64 = [&](int c, float (&v)[64]) {
+          uint32_t e[2][32];
+          tmem_ld32(acc + c, e[0]);
+          tmem_ld32(acc + c + 32, e[1]);
+          tmem_wait();
+          finish32(e[0], v, pr + c, sa, B200DEC_ACT_NONE);
+          finish32(e[1], v + 32, pr + c + 32, sa, B200DEC_ACT_NONE);
+        };
+#pragma unroll 1
+        for (int c = 0; c < HALF; c += 64) {
+          const int n = n0 + c, hd = p.H * p.D, l = n / (2 * hd), kvi = (n / hd) & 1, h = (n % hd) / p.D, d0 = n % p.D;
+          const size_t vec = slot < 0 ? 0 : ((((size_t)l * p.S1 + slot) * p.H + h) * p.T + frame);
+          float v[64];
+          load64(c, v);
+          if (p.mode == 1) {
+            if (slot >= 0) {
+              __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(kvi ? p.cv : p.ck) + vec * p.D + d0;
+#pragma unroll
+              for (int i = 0; i < 64; i += 8)
+                *reinterpret_cast<uint4*>(dst + i) = make_uint4(pack_bf16(v[i], v[i + 1]), pack_bf16(v[i + 2], v[i + 3]),
+                                                                pack_bf16(v[i + 4], v[i + 5]), pack_bf16(v[i + 6], v[i + 7]));
+            }
+          } else if (p.mode == 3) {
+            if (slot >= 0)
+              store_q4_64(v, reinterpret_cast<uint8_t*>(kvi ? p.cv : p.ck) + (vec * p.D + d0) / 2,
+                          reinterpret_cast<uint32_t*>(kvi ? p.cvs : p.cks) + (vec * p.D + d0) / 64);
+          } else {
+            // int8: the vector's largest magnitude over its 64 or 128 channels (a half of the columns holds a whole vector)
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) {
+              v[i] = __bfloat162float(__float2bfloat16_rn(v[i]));
+              mx = fmaxf(mx, fabsf(v[i]));
+            }
+            int8_t* dst = reinterpret_cast<int8_t*>(kvi ? p.cv : p.ck) + vec * p.D + d0;
+            if (p.D == 128) {
+              float u[64];
+              load64(c + 64, u);
+#pragma unroll
+              for (int i = 0; i < 64; ++i) {
+                u[i] = __bfloat162float(__float2bfloat16_rn(u[i]));
+                mx = fmaxf(mx, fabsf(u[i]));
+              }
+              if (slot >= 0) store_q8_64(u, mx, dst + 64);
+              c += 64;
+            }
+            if (slot >= 0) {
+              store_q8_64(v, mx, dst);
+              (kvi ? p.cvs : p.cks)[vec] = mx > 0.f ? __fdiv_rn(mx, 127.f) : 1.f;
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[buf]);
+    }
+    if (!ok && lane == 0) atomicOr(p.status, B200DEC_ST_TIMEOUT);
+  }
+  // ---- release the tensor memory: after every warp is done with it -----------------------------------------------------
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "n"(Cfg::TMEM_COLS) : "memory");
+  }
+}
+
+// ---- 8-bit operands --------------------------------------------------------------------------------------------------------
+// Rows -> 8-bit integers with one scale a row: s = max(max |x|, 1e-12) / 127, q = rint(x / s), both as if the quotients were
+// exact: the product with the reciprocal is off by a few 2^-23 of it, so only its rounding beside a half can be wrong, and
+// the remainder x - q s (exact: a multiple of ulp(s) / 2 below 2^24 of them) decides there. A row with an infinity or NaN gets
+// scale NaN: its results are NaN. One warp a row, which passes over it twice (the second time out of L1 and L2).
+template <class X>
+DEVI float row_value(X x) {
+  if constexpr (std::is_same<X, float>::value) return x;
+  else if constexpr (std::is_same<X, __half>::value) return __half2float(x);
+  else return __bfloat162float(x);
+}
+
+// values c .. c + 15 of a row of k, zeros past its end
+template <class X, bool WIDE>
+DEVI void load_16(const X* row, int c, int k, float (&f)[16]) {
+  if (WIDE && c + 16 <= k) {
+    constexpr int PER = 16 / (int)sizeof(X);
+#pragma unroll
+    for (int i = 0; i < 16 / PER; ++i) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+      X x[PER];
+      memcpy(x, &w, 16);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) f[i * PER + j] = row_value(x[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = c + i < k ? row_value(row[c + i]) : 0.f;
+  }
+}
+
+DEVI int code8(float x, float s, float inv) {
+  float c = fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
+  const float e2 = 2.f * __fmaf_rn(-c, s, x);
+  const bool odd = ((int)c & 1) != 0;
+  if (e2 > s || (e2 == s && odd)) c += 1.f;
+  if (-e2 > s || (-e2 == s && odd)) c -= 1.f;
+  return (int)fminf(fmaxf(c, -127.f), 127.f);
+}
+
+template <class X, bool WIDE>
+__global__ void __launch_bounds__(256) pack_rows_i8_kernel(const X* __restrict__ x, int m, int k, int64_t ldx,
+                                                           unsigned char* __restrict__ image, float* __restrict__ scale) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  if (row >= m) return;  // the rows that fill the last tile up are never stored: whatever the image holds there does no harm
+  const X* src = x + row * ldx;
+  uint32_t top = 0;  // largest magnitude by its bits, so that a NaN is the largest
+  for (int c = lane * 16; c < k; c += 512) {
+    float f[16];
+    load_16<X, WIDE>(src, c, k, f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float s = top < 0x7f800000u ? __fdiv_rn(fmaxf(__uint_as_float(top), 1e-12f), 127.f) : __uint_as_float(0x7fffffffu);
+  const float inv = __frcp_rn(s);
+  if (lane == 0) scale[row] = s;
+  const int kp = (k + 127) / 128 * 128;
+  unsigned char* tile = image + (size_t)(row / BM) * (kp / 128) * A_STAGE;
+  for (int c = lane * 16; c < kp; c += 512) {
+    float f[16];
+    load_16<X, WIDE>(src, c, k, f);
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i >> 2] |= (uint32_t)(code8(f[i], s, inv) & 0xff) << ((i & 3) * 8);
+    *reinterpret_cast<uint4*>(tile + (size_t)(c / 128) * A_STAGE + swz(row % BM, (c % 128) / 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// int8 weights (n, k) row-major -> [n / 256][k / 128][256 rows x 128 B, swizzled], zeros where n or k end; a thread per 16 bytes
+__global__ void tile_weight_i8_kernel(const int8_t* __restrict__ q, int n, int k, unsigned char* __restrict__ out) {
+  const int np = (n + BN - 1) / BN * BN, kp = (k + 127) / 128 * 128, cpr = kp / 16;
+  const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= (size_t)np * cpr) return;
+  const int r = (int)(i / cpr), c = (int)(i % cpr);
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (r < n && c * 16 + j < k) w[j >> 2] |= (uint32_t)(uint8_t)q[(size_t)r * k + c * 16 + j] << ((j & 3) * 8);
+  *reinterpret_cast<uint4*>(out + ((size_t)(r / BN) * (kp / 128) + c / 8) * B_BLOCK + swz(r % BN, c % 8)) =
+      make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <class X>
+cudaError_t launch_pack_i8(const void* x, int m, int k, int64_t ldx, void* image, float* scale, cudaStream_t st) {
+  const bool wide = ((uintptr_t)x & 15) == 0 && (m == 1 || ldx * sizeof(X) % 16 == 0);
+  const dim3 grid((m + 7) / 8);
+  if (wide) pack_rows_i8_kernel<X, true><<<grid, 256, 0, st>>>((const X*)x, m, k, ldx, (unsigned char*)image, scale);
+  else pack_rows_i8_kernel<X, false><<<grid, 256, 0, st>>>((const X*)x, m, k, ldx, (unsigned char*)image, scale);
+  return cudaGetLastError();
+}
+
+template <int TN>
+int launch_tile(const W8Args& a, int sms, cudaStream_t stream) {
+  constexpr int BYTES = Tile<TN>::SMEM_BYTES;
+  cudaError_t e = cudaFuncSetAttribute(w8a8_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+  if (e != cudaSuccess) return fail(B200DEC_ECUDA, "w8a8: smem attribute: %s", cudaGetErrorString(e));
+  const int64_t tiles = (int64_t)((a.M + BM - 1) / BM) * ((a.N + TN - 1) / TN);
+  e = launch_kernel(w8a8_kernel<TN>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(NTHREADS), BYTES, stream, 0, true, a);
+  if (e != cudaSuccess) return fail(B200DEC_ECUDA, "w8a8 launch: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+// The narrowest tile with which the tiles still are one wave, else the widest: the wide one copies least per product.
+int launch(const W8Args& a, cudaStream_t stream) {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t mt = (a.M + BM - 1) / BM;
+  if (a.mode == 4 && mt * ((a.N + 63) / 64) <= sms) return launch_tile<64>(a, sms, stream);
+  if (a.mode == 4 && mt * ((a.N + 127) / 128) <= sms) return launch_tile<128>(a, sms, stream);
+  return launch_tile<256>(a, sms, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t b200dec_w8a8_rows_bytes(int m, int k) {
+  if (m < 0 || k <= 0 || k > MAX_K8) return -1;
+  return (int64_t)((m + BM - 1) / BM) * BM * ((k + 127) / 128 * 128);
+}
+
+int64_t b200dec_w8a8_weight_bytes(int n, int k) {
+  if (n <= 0 || k <= 0 || k > MAX_K8) return -1;
+  return (int64_t)((n + BN - 1) / BN) * BN * ((k + 127) / 128 * 128);
+}
+
+int b200dec_w8a8_pack_rows(const void* x, int kind, int m, int k, int64_t ldx, void* image, float* scale, void* stream) {
+  B200_REQUIRE(x && image && scale, "w8a8_pack_rows: null pointer");
+  B200_REQUIRE(m >= 1 && k >= 1 && k <= MAX_K8 && (m == 1 || ldx >= k), "w8a8_pack_rows: m %d k %d ldx %lld", m, k, (long long)ldx);
+  B200_REQUIRE(kind == B200DEC_T_F32 || kind == B200DEC_T_F16 || kind == B200DEC_T_BF16, "w8a8_pack_rows: kind %d", kind);
+  B200_REQUIRE(((uintptr_t)image & 1023) == 0 && (uintptr_t)x % (kind == B200DEC_T_F32 ? 4 : 2) == 0,
+               "w8a8_pack_rows: alignment (the image 1 KB)");
+  const cudaStream_t st = (cudaStream_t)stream;
+  const cudaError_t e = kind == B200DEC_T_F32   ? launch_pack_i8<float>(x, m, k, ldx, image, scale, st)
+                        : kind == B200DEC_T_F16 ? launch_pack_i8<__half>(x, m, k, ldx, image, scale, st)
+                                                : launch_pack_i8<__nv_bfloat16>(x, m, k, ldx, image, scale, st);
+  if (e != cudaSuccess) return fail(B200DEC_ECUDA, "w8a8_pack_rows launch: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+int b200dec_w8a8_tile_weight(const int8_t* q, int n, int k, void* image, void* stream) {
+  B200_REQUIRE(q && image && n >= 1 && k >= 1 && k <= MAX_K8 && ((uintptr_t)image & 1023) == 0,
+               "w8a8_tile_weight: (%d, %d) into a 1 KB aligned image", n, k);
+  const size_t total = (size_t)b200dec_w8a8_weight_bytes(n, k) / 16;
+  tile_weight_i8_kernel<<<(unsigned)((total + 255) / 256), 256, 0, (cudaStream_t)stream>>>(q, n, k, (unsigned char*)image);
+  return check_launch("w8a8_tile_weight");
+}
+
+int b200dec_w8a8_linear(const void* rows_image, const float* row_scale, int m, int k, const void* weight_image,
+                        const float* w_scale, const float* bias, int n, int act, void* out, int out_kind, int64_t ldo,
+                        int32_t* status, void* stream) {
+  B200_REQUIRE(rows_image && row_scale && weight_image && w_scale && out && status, "w8a8_linear: null pointer");
+  B200_REQUIRE(m >= 1 && n >= 1 && k >= 1 && k <= MAX_K8 && (m == 1 || ldo >= n), "w8a8_linear: m %d k %d n %d ldo %lld", m, k, n,
+               (long long)ldo);
+  B200_REQUIRE(out_kind == B200DEC_T_F32 || out_kind == B200DEC_T_F16 || out_kind == B200DEC_T_BF16, "w8a8_linear: out_kind %d", out_kind);
+  B200_REQUIRE(act == B200DEC_ACT_NONE || act == B200DEC_ACT_RELU || act == B200DEC_ACT_GELU, "w8a8_linear: act %d", act);
+  B200_REQUIRE((((uintptr_t)rows_image | (uintptr_t)weight_image) & 1023) == 0 && (((uintptr_t)w_scale | (uintptr_t)bias) & 15) == 0 &&
+                   (uintptr_t)out % (out_kind == B200DEC_T_F32 ? 4 : 2) == 0,
+               "w8a8_linear: alignment (images 1 KB, channel scales and bias 16 bytes)");
+  W8Args a{};
+  a.a = (const unsigned char*)rows_image, a.w = (const unsigned char*)weight_image, a.bias = bias;
+  a.M = m, a.N = n, a.NKB = (k + 127) / 128, a.mode = 4, a.status = status;
+  a.a_scale = row_scale, a.w_scale = w_scale, a.out = out, a.ldo = ldo, a.out_kind = out_kind, a.act = act;
+  return launch(a, (cudaStream_t)stream);
+}
+
+int b200dec_w8a8_prefill(const void* rows_image, const float* row_scale, int m, int k, const void* weight_image,
+                         const float* w_scale, const float* bias, int n, int mode, const int32_t* pieces, int n_pieces, void* ck,
+                         void* cv, void* ck_scale, void* cv_scale, int layers, int slots_plus_1, int heads, int head_dim, int frames,
+                         int32_t* status, void* stream) {
+  B200_REQUIRE(rows_image && row_scale && weight_image && w_scale && status, "w8a8_prefill: null pointer");
+  B200_REQUIRE(m >= 1 && k >= 1 && k <= MAX_K8 && mode >= 1 && mode <= 3, "w8a8_prefill: m %d k %d mode %d", m, k, mode);
+  B200_REQUIRE(pieces && n_pieces >= 1 && ck && cv && (mode == 1 || (ck_scale && cv_scale)), "w8a8_prefill: pieces and caches");
+  B200_REQUIRE((((uintptr_t)rows_image | (uintptr_t)weight_image) & 1023) == 0 &&
+                   (((uintptr_t)w_scale | (uintptr_t)bias | (uintptr_t)pieces | (uintptr_t)ck | (uintptr_t)cv) & 15) == 0,
+               "w8a8_prefill: alignment (images 1 KB, the rest 16 bytes)");
+  B200_REQUIRE((head_dim == 64 || head_dim == 128) && layers >= 1 && heads >= 1 && slots_plus_1 >= 1 && frames >= 1 &&
+                   (int64_t)n == (int64_t)layers * 2 * heads * head_dim && n % BN == 0,
+               "w8a8_prefill: n %d != layers %d x 2 x heads %d x head_dim %d (a multiple of 256)", n, layers, heads, head_dim);
+  W8Args a{};
+  a.a = (const unsigned char*)rows_image, a.w = (const unsigned char*)weight_image, a.bias = bias;
+  a.M = m, a.N = n, a.NKB = (k + 127) / 128, a.mode = mode, a.status = status, a.a_scale = row_scale, a.w_scale = w_scale;
+  a.pieces = (const int4*)pieces, a.n_pieces = n_pieces, a.ck = ck, a.cv = cv, a.cks = (float*)ck_scale, a.cvs = (float*)cv_scale;
+  a.S1 = slots_plus_1, a.H = heads, a.D = head_dim, a.T = frames;
+  return launch(a, (cudaStream_t)stream);
+}
+
+}  // extern "C"
