@@ -53,33 +53,68 @@ DEVI size_t vec_of(const Kv4Args& p, const Channel& c, int slot, int frame) {
 }
 DEVI bool inside(const Kv4Args& p, int slot, int frame) { return slot >= 0 && slot < p.S1 && frame >= 0 && frame < p.T; }
 
+// The extremes of a thread's 8 values go round in bf16, the largest and the negated smallest in one word.
+DEVI uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2_nan(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
+  return reinterpret_cast<const uint32_t&>(m);
+}
+DEVI uint32_t min_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmin2_nan(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
+  return reinterpret_cast<const uint32_t&>(m);
+}
+
 __global__ void __launch_bounds__(THREADS) scatter_kv_q4_kernel(const Kv4Args p) {
   const Channel c = channel(p);
   const size_t width = (size_t)p.L * 2 * p.H * p.D, at = (size_t)(blockIdx.x * THREADS + threadIdx.x) * 8;
-  for (int row = blockIdx.y; row < p.nrows; row += gridDim.y) {
-    const int slot = __ldg(p.slot_of + row), frame = __ldg(p.frame_of + row);
-    if (!inside(p, slot, frame)) continue;  // the whole CTA
+  const auto load = [&](int row, int& slot, int& frame) {
+    slot = -1, frame = 0;
     f32x8 x{};
-    if (c.live) x = ld_stream32(p.kv + row * width + at);
-    float mn = INFINITY, mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const uint32_t w = pack_bf16(x.v[i], x.v[i + 1]);
-      x.v[i] = kv4_clamp(bf16_lo(w)), x.v[i + 1] = kv4_clamp(bf16_hi(w));
-      mn = fminf(mn, fminf(x.v[i], x.v[i + 1])), mx = fmaxf(mx, fmaxf(x.v[i], x.v[i + 1]));
+    if (row < p.nrows) {
+      slot = __ldg(p.slot_of + row), frame = __ldg(p.frame_of + row);
+      if (c.live) x = ld_stream32(p.kv + row * width + at);
     }
+    return x;
+  };
+  int slot, frame;
+  f32x8 now = load(blockIdx.y, slot, frame);
+  for (int row = blockIdx.y; row < p.nrows; row += gridDim.y) {
+    const int s = slot, f = frame;
+    f32x8 x = now;
+    now = load(row + gridDim.y, slot, frame);  // the next row is on its way while this one is worked on
+    if (!inside(p, s, f)) continue;  // the whole CTA
+    uint32_t w[4];
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16(x.v[2 * i], x.v[2 * i + 1]);
+    const uint32_t hi = max_bf16x2(max_bf16x2(w[0], w[1]), max_bf16x2(w[2], w[3]));
+    const uint32_t lo = min_bf16x2(min_bf16x2(w[0], w[1]), min_bf16x2(w[2], w[3]));
+    // {largest, -smallest} of the 8, then of the group
+    uint32_t ext = max_bf16x2(__byte_perm(hi, lo ^ 0x80008000u, 0x5410), __byte_perm(hi, lo ^ 0x80008000u, 0x7632));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) ext = max_bf16x2(ext, __shfl_xor_sync(0xffffffffu, ext, o));
+    float mx = bf16_lo(ext), mn = -bf16_hi(ext);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.v[2 * i] = bf16_lo(w[i]), x.v[2 * i + 1] = bf16_hi(w[i]);
+    const bool tame = mx <= KV4_LIMIT && mn >= -KV4_LIMIT;  // false for a NaN too
+    if (__any_sync(0xffffffffu, !tame)) {  // something to clamp, or a NaN, in some group of the warp
+      mn = INFINITY, mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.v[i] = kv4_clamp(x.v[i]), mn = fminf(mn, x.v[i]), mx = fmaxf(mx, x.v[i]);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      }
     }
     if (!c.live) continue;
     const Kv4Group g = kv4_group(mn, mx);
-    uint32_t w = 0;
+    uint32_t codes = 0;
+    if (kv4_plain(g)) codes = kv4_codes8(x.v, g);
+    else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= (uint32_t)kv4_code(x.v[i], g) << (4 * i);
-    const size_t vec = vec_of(p, c, slot, frame);
-    (c.kvi ? p.cv : p.ck)[vec * (p.D / 8) + c.d8] = w;
+      for (int i = 0; i < 8; ++i) codes |= (uint32_t)kv4_code(x.v[i], g) << (4 * i);
+    }
+    const size_t vec = vec_of(p, c, s, f);
+    (c.kvi ? p.cv : p.ck)[vec * (p.D / 8) + c.d8] = codes;
     if ((c.d8 & 7) == 0) (c.kvi ? p.cvm : p.ckm)[vec * (p.D / 64) + (c.d8 >> 3)] = g.word;
   }
 }

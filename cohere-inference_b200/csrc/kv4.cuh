@@ -43,6 +43,29 @@ DEVI int kv4_code(float x, const Kv4Group& g) {
   if (-e2 > g.step || (-e2 == g.step && odd)) c -= 1.f;
   return g.step > 0.f ? (int)fminf(fmaxf(c, 0.f), 15.f) : 0;
 }
+// The group's pair and 8 of its values' codes, of values that are finite and within the limit, where |lo| <= 512 steps and the step
+// is a normal fp16 number (else false: the caller takes kv4_code for each). Then 0 <= x - lo + step / 2 and (x - lo) / step <=
+// 15.01, so nothing has to be clamped, and only a quotient within 2^-17 of a half needs the exact remainder. Adding 1.5 * 2^23
+// rounds to an integer, which the sum's low bits are.
+DEVI bool kv4_plain(const Kv4Group& g) { return g.step >= 6.103515625e-05f && fabsf(g.lo) <= 512.f * g.step; }
+DEVI uint32_t kv4_codes8(const float (&x)[8], const Kv4Group& g) {
+  constexpr float MAGIC = 12582912.f;  // 0x4b400000
+  uint32_t w = 0;
+  float near = 0.f;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    const float d = x[i] - g.lo, t = __fmaf_rn(d, g.inv, MAGIC);
+    near = fmaxf(near, fabsf(__fmaf_rn(d, g.inv, MAGIC - t)));
+    w = w * 16u + __float_as_uint(t);
+  }
+  w -= 0x4b400000u * 0x11111111u;
+  if (near > 0.5f - 7.62939453e-06f) {
+    w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= (uint32_t)kv4_code(x[i], g) << (4 * i);
+  }
+  return w;
+}
 DEVI float kv4_value(int code, float step, float lo) { return __fmaf_rn((float)code, step, lo); }
 
 }  // namespace b200dec_detail
