@@ -27,6 +27,9 @@ int pick_impl(const float* part_max, const int32_t* part_idx, int partials, cons
 int attention_spans_impl(int self, const int32_t* sched, const float* q, int ldq, void* kcache, void* vcache, float* kscale,
                          float* vscale, int heads, int head_dim, int cap, float scale, void* out, int out_kind, int rows,
                          int64_t step_items, int pdl, void* stream);
+int logit_rules_impl(const void* logits, int kind, int64_t ldl, int rows, int vocab, const int32_t* active, int slots,
+                     const b200dec_rules* rules, void* out, int64_t ldo, float* best, int32_t* token, int32_t* status, int pdl,
+                     void* stream);
 bool fused_step_applies(const b200dec_plan* pl, int row0, int rows);
 int fused_step(const b200dec_plan* pl, int rows, void* stream);
 }  // namespace b200dec_detail
@@ -65,7 +68,7 @@ int b200dec_step_launches(const b200dec_plan* pl, int rows) {
   if (fused_step_applies(pl, 0, rows)) return 1;
   const bool linked = pl->xh && pl->ln_stats && pl->a_kind == B200DEC_A_F16 && pl->layer[0].qkv.kind != B200DEC_W_BF16;
   const int ln_kind = linked ? B200DEC_A_F16_ROWS16 : pl->a_kind;
-  int n = 2;  // embedding, pick
+  int n = pl->rules ? 3 : 2;  // embedding, pick, and the rules on the logits
   for (int i = 0; i < pl->layers; ++i) {
     const b200dec_layer& ly = pl->layer[i];
     n += 2 + linear_passes(&ly.qkv, ln_kind, true, rows) + linear_passes(&ly.o, pl->a_kind, false, rows) +
@@ -86,6 +89,8 @@ int b200dec_step_part(const b200dec_plan* pl, int row0, int rows, int step_rows,
   B200_REQUIRE(pl->heads * pl->head_dim == D_MODEL, "step: heads * head_dim must be %d", D_MODEL);
   B200_REQUIRE(pl->vocab == pl->head.n, "step: vocab %d vs head rows %d", pl->vocab, pl->head.n);
   B200_REQUIRE(!(pl->kv_int8 && pl->attn_ring), "step: the ring attention kernel reads bf16 caches only");
+  B200_REQUIRE(!pl->kv_int4 || !(pl->kv_int8 || pl->attn_ring), "step: 4-bit caches are a mode of their own");
+  B200_REQUIRE(!pl->rules || (pl->logits && pl->rule_best && pl->rule_token), "step: rules need the logits and a place for the choice");
   if (fused_step_applies(pl, row0, rows)) return fused_step(pl, rows, stream);  // up to 16 rows: one kernel (step_fused.cuh)
   const int hd = pl->heads * pl->head_dim;
   const int want = pl->classes ? pl->classes : 7;  // 1 embedding / vocabulary projection / pick, 2 projections, 4 attention
@@ -161,14 +166,15 @@ int b200dec_step_part(const b200dec_plan* pl, int row0, int rows, int step_rows,
   // caches, 574 / 535, 658 / 590, 729 / 647. Where the whole is not known (step_rows 0): as if alone, but paired from 512 items.
   const int items = rows * pl->heads, step_items = step_rows ? step_rows * pl->heads : items;
   const bool ranked = !pl->attn_ring && pl->sched_self && pl->sched_cross && items >= 128 && rows <= 256;
-  const bool paired = ranked && items == step_items && items >= (step_rows ? 4 * 148 : 512) && items <= 7 * 148;
-  const bool spans = ranked && !paired;
+  // 4-bit caches have one kernel for all of this: it takes the ranked rows as they come and chooses its CTAs by itself.
+  const bool paired = ranked && !pl->kv_int4 && items == step_items && items >= (step_rows ? 4 * 148 : 512) && items <= 7 * 148;
+  const bool spans = ranked && !pl->kv_int4 && !paired;
   int32_t* sched_self = ranked ? pl->sched_self + 4 * row0 : nullptr;
   int32_t* sched_cross = ranked ? pl->sched_cross + 4 * row0 : nullptr;
 
   // Prefetch of the attention launches' caches into L2 by the output projections (common.cuh, KvPrefetch): the budget
   // in keys per launch; one key of a row is 2 (key, value) x heads x vec_bytes bytes.
-  const int vec_bytes = pl->head_dim * (pl->kv_int8 ? 1 : 2);
+  const int vec_bytes = pl->kv_int4 ? pl->head_dim / 2 : pl->head_dim * (pl->kv_int8 ? 1 : 2);
   const int prefetch_keys =
       ranked && items >= 512 && pl->kv_prefetch_mb > 0 ? (int)(((long long)pl->kv_prefetch_mb << 20) / (2LL * pl->heads * vec_bytes)) : 0;
   auto prefetch = [&](const int32_t* sched, const void* k, const void* v, int cap) {
@@ -177,6 +183,15 @@ int b200dec_step_part(const b200dec_plan* pl, int row0, int rows, int step_rows,
       f = KvPrefetch{reinterpret_cast<const int4*>(sched), (const char*)k, (const char*)v, rows, pl->heads, cap, vec_bytes,
                      pl->slots};
     return f;
+  };
+
+  const auto attention_q4 = [&](int self, const int32_t* sched, const float* q, int ldq, void* k, void* v, void* kp, void* vp,
+                                const int32_t* len, int cap, int pdl_) {
+    const bool room = b200dec_attention_q4_scratch_floats(rows, pl->heads, pl->head_dim, cap) <=
+                      b200dec_attention_scratch_floats(rows, pl->heads, pl->head_dim);
+    return b200dec_attention_q4(self, active, q, ldq, k, v, kp, vp, len, sched, pl->slots, pl->heads, pl->head_dim, cap, scale, att,
+                                ok_a, rows, room ? attn_part : nullptr, room && attn_part ? attn_count : nullptr, pl->status, pdl_,
+                                stream);
   };
 
   B200_TRY_IN(1, embed_ln_impl(active, pl->tok, pl->pos, pl->embed, pl->pos_table, pl->vocab, pl->max_pos, pl->slots,
@@ -202,7 +217,9 @@ int b200dec_step_part(const b200dec_plan* pl, int row0, int rows, int step_rows,
     // projections left out (classes) the first self-attention would follow the embedding directly and the two CTAs of
     // a pair could see different versions of an entry and disagree on their hand-off: it is then launched plainly.
     const int pdl_self = (i == 0 && !(want & 2)) ? 0 : pdl_attn;
-    if (spans)
+    if (pl->kv_int4)
+      B200_TRY_IN(4, attention_q4(1, sched_self, qkv, 3 * hd, ly.self_k, ly.self_v, ly.self_ks, ly.self_vs, pl->pos, pl->seq, pdl_self));
+    else if (spans)
       B200_TRY_IN(4, attention_spans_impl(1, sched_self, qkv, 3 * hd, ly.self_k, ly.self_v,
                                              pl->kv_int8 ? ly.self_ks : nullptr, pl->kv_int8 ? ly.self_vs : nullptr,
                                              pl->heads, pl->head_dim, pl->seq, scale, att, ok_a, rows, step_items,
@@ -225,7 +242,10 @@ int b200dec_step_part(const b200dec_plan* pl, int row0, int rows, int step_rows,
                          pdl_after, stream, &p2, &f_cross));
     B200_TRY_IN(2, linear_impl(&ly.cq, ln_src, ln_kind, &ly.ln2, D_MODEL, rows, cq, B200DEC_OUT_F32, hd, B200DEC_ACT_NONE, pdl,
                          stream, &r2, nullptr));
-    if (spans)
+    if (pl->kv_int4)
+      B200_TRY_IN(4, attention_q4(0, sched_cross, cq, hd, (void*)ly.cross_k, (void*)ly.cross_v, ly.cross_ks, ly.cross_vs, pl->cross_len,
+                                  pl->frames, pdl_attn));
+    else if (spans)
       B200_TRY_IN(4, attention_spans_impl(0, sched_cross, cq, hd, (void*)ly.cross_k, (void*)ly.cross_v,
                                              pl->kv_int8 ? ly.cross_ks : nullptr, pl->kv_int8 ? ly.cross_vs : nullptr,
                                              pl->heads, pl->head_dim, pl->frames, scale, att, ok_a, rows,
@@ -260,7 +280,15 @@ int b200dec_step_part(const b200dec_plan* pl, int row0, int rows, int step_rows,
   else
     B200_TRY_IN(1, head_impl(&pl->head, x, pl->head_a_kind, &pl->final_ln, D_MODEL, rows, head_max, head_idx, logits, pdl,
                        stream));
-  B200_TRY_IN(1, pick_impl(head_max, head_idx, partials, active, rows, pl->slots, pl->tok, pl->pos, pl->finished, pl->forced,
+  // under rules the row's choice is theirs, one partial per row
+  const float* pick_max = head_max;
+  const int32_t* pick_idx = head_idx;
+  if (pl->rules) {
+    B200_TRY_IN(1, logit_rules_impl(logits, B200DEC_T_F32, pl->vocab, rows, pl->vocab, active, pl->slots, pl->rules, nullptr, 0,
+                                    pl->rule_best + row0, pl->rule_token + row0, pl->status, pdl, stream));
+    pick_max = pl->rule_best + row0, pick_idx = pl->rule_token + row0;
+  }
+  B200_TRY_IN(1, pick_impl(pick_max, pick_idx, pl->rules ? 1 : partials, active, rows, pl->slots, pl->tok, pl->pos, pl->finished, pl->forced,
                      pl->max_prompt, pl->plen, pl->limit, pl->out, pl->out_cols, pl->eos, pl->argmax, pl->flags_host, pdl,
                            stream));
   return 0;

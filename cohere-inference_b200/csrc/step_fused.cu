@@ -22,7 +22,7 @@ bool all_kinds(const b200dec_plan* pl, int attn, int ffn) {
 
 // the kernel's weight mode for this plan and row count, or -1
 int fused_mode(const b200dec_plan* pl, int rows) {
-  if (rows < 1 || rows > F_MAX_ROWS || pl->layers > F_MAX_LAYERS || pl->attn_ring) return -1;
+  if (rows < 1 || rows > F_MAX_ROWS || pl->layers > F_MAX_LAYERS || pl->attn_ring || pl->kv_int4 || pl->rules) return -1;
   if (!((pl->heads == 16 && pl->head_dim == 64) || (pl->heads == 8 && pl->head_dim == 128))) return -1;
   const b200dec_weight& h = pl->head;
   if (!h.ln_g || !h.ln_bias || h.k != D_MODEL || h.n != pl->vocab || pl->vocab % 16) return -1;

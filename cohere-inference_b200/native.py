@@ -45,6 +45,11 @@ class Layer(C.Structure):
                 ("cross_v", vp), ("self_ks", vp), ("self_vs", vp), ("cross_ks", vp), ("cross_vs", vp)]
 
 
+class Rules(C.Structure):
+    _fields_ = [("params", vp), ("history", vp), ("last", vp), ("plen", vp), ("bias_ids", vp), ("bias", vp), ("bias_n", vp),
+                ("mask", vp), ("mask_on", vp), ("hist_cols", i32), ("max_bias", i32)]
+
+
 class Plan(C.Structure):
     _fields_ = [("layers", i32), ("heads", i32), ("head_dim", i32), ("act", i32),
                 ("slots", i32), ("seq", i32), ("frames", i32), ("vocab", i32),
@@ -58,12 +63,8 @@ class Plan(C.Structure):
                 ("x", vp), ("qkv", vp), ("cq", vp), ("att", vp), ("mid", vp),
                 ("attn_part", vp), ("attn_count", vp), ("head_max", vp), ("head_idx", vp),
                 ("xh", vp), ("ln_stats", vp), ("sched_self", vp), ("sched_cross", vp), ("logits", vp), ("argmax", vp),
-                ("fused_ws", vp * 16)]
-
-
-class Rules(C.Structure):
-    _fields_ = [("params", vp), ("history", vp), ("last", vp), ("plen", vp), ("bias_ids", vp), ("bias", vp), ("bias_n", vp),
-                ("mask", vp), ("mask_on", vp), ("hist_cols", i32), ("max_bias", i32)]
+                ("fused_ws", vp * 16), ("kv_int4", i32), ("_pad2", i32), ("rules", C.POINTER(Rules)), ("rule_best", vp),
+                ("rule_token", vp)]
 
 
 # name -> (restype, argtypes); every symbol include/b200dec.h declares

@@ -167,9 +167,12 @@ class DecodeScheduler:
             if new_idx:
                 new_reqs = [requests[i] for i in new_idx]
                 self._fill(new_reqs, new_slots)
+                # a request may carry rules for the choice of its tokens (StreamDecoder.admit)
+                rules = [getattr(r, "rules", None) for r in new_reqs]
                 dec.admit(new_slots, [torch.as_tensor(r.prompt) if self.cuda else r.prompt for r in new_reqs],
                           [r.frames for r in new_reqs],
-                          [min(getattr(r, "target", dec.max_new_tokens), dec.max_new_tokens) for r in new_reqs])
+                          [min(getattr(r, "target", dec.max_new_tokens), dec.max_new_tokens) for r in new_reqs],
+                          **({"rules": rules} if any(x is not None for x in rules) else {}))
                 for s, i in zip(new_slots, new_idx):
                     req_of[s], admitted_at[s], pos_of[s] = i, step_no, 0
                 active += new_slots

@@ -25,7 +25,7 @@ import numpy as np
 import torch
 
 from . import native as nv
-from .packing import PackedLinear, dequantized, pack_linear
+from .packing import PackedLinear, dequantized, pack_linear, quantize_rows
 
 ACTS = {"relu": nv.ACT_RELU, "gelu": nv.ACT_GELU}
 
@@ -87,6 +87,18 @@ class _PrefillWeight:
         self.bias[:n] = b.detach().float()
 
 
+class _PrefillWeightInt8:
+    """The same projection in 8 bits (csrc/w8a8.cu): quantize_rows' values and scales, the rows quantised as they come."""
+
+    def __init__(self, w: torch.Tensor, b: torch.Tensor):
+        self.n, self.k = w.shape
+        q, self.scale = quantize_rows(w)
+        self.image = nv.image(nv.lib().b200dec_w8a8_weight_bytes(self.n, self.k), w.device)
+        nv.check(nv.lib().b200dec_w8a8_tile_weight(nv.ptr(q), self.n, self.k, nv.ptr(self.image), nv.stream_ptr()))
+        torch.cuda.current_stream().synchronize()
+        self.bias = b.detach().float().contiguous()
+
+
 class StreamDecoder:
     BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 80, 96, 112, 128)
 
@@ -96,7 +108,8 @@ class StreamDecoder:
                  head_split: bool = True, keep_reference: bool = False, chains: int = 1, attn_ring: bool = False,
                  head_umma: bool = True, kv_int8: bool = False, proj_umma: bool | str = True,
                  kv_prefetch_mb: int = 0, device_sched: bool = False, fp16_weights: bool = False,
-                 umma_above_rows: int = 16, fused_rows: int = 16,
+                 umma_above_rows: int = 16, fused_rows: int = 16, kv_int4: bool = False, prefill_int8: bool = False,
+                 logit_rules: bool = False, max_bias: int = 64,
                  _packed: tuple | None = None):
         """model: a CohereAsrForConditionalGeneration-shaped module on a CUDA device (see synth.synthetic_model).
         int8: weight-only int8 with per-output-channel scales on every projection (fp16 activations, fp32
@@ -120,10 +133,17 @@ class StreamDecoder:
         (0: tcgen05 in every bucket). fused_rows: buckets of up to this many rows (at most 16) run a step as one
         cooperative kernel where the mode has it and it is the faster way (csrc/step_fused.cu; 0: as the sequence of
         kernels). The fused steps of several decoders on one GPU take turns; a step that is captured by the caller
-        (graphs=False) is always the sequence."""
+        (graphs=False) is always the sequence. kv_int4: keys and values in 4 bits with an fp16 pair per 64 dims, 4.5 bits
+        a value (csrc/kv4.cuh). prefill_int8: the two products of fill_cross in 8-bit integers, weights per channel and rows
+        as they come (csrc/w8a8.cu). logit_rules: every slot has penalties for repeated tokens, up to max_bias biases and a
+        mask over the vocabulary, given with `admit` and `set_mask`, under which the greedy choice is made
+        (csrc/logit_rules.cu). Steps with kv_int4 or logit_rules are the sequence of kernels at every size."""
         nv.lib()  # fail now, loudly, if the CUDA library is missing
         assert not ffn_sparse or int8, "2:4 feed-forward weights are int8"
         assert not (fp16_weights and int8), "fp16_weights is a mode of its own beside int8"
+        assert not kv_int4 or not (kv_int8 or attn_ring), "kv_int4 is a mode of its own beside kv_int8 and the ring kernel"
+        if logit_rules and not 1 <= max_bias <= 1024:
+            raise ValueError("max_bias: 1..1024 biases per slot")
         cfg = model.config
         dev = model.device if _packed else model.model.decoder.embed_tokens.weight.device
         assert dev.type == "cuda", "StreamDecoder needs the model on a CUDA device: there is no CPU path"
@@ -164,6 +184,9 @@ class StreamDecoder:
             self._pack_options = dict(int8=bool(int8), fp16_weights=bool(fp16_weights), ffn_sparse=bool(ffn_sparse),
                                       head_split=bool(head_split), head_umma=bool(head_umma),
                                       proj_umma=",".join(sorted(umma)), max_rows=bm, small_rows=self._small_rows)
+            self.prefill_int8 = bool(prefill_int8)
+            if self.prefill_int8:
+                self._pack_options["prefill_int8"] = True
             if _packed:
                 self._load_packed(*_packed)
             else:
@@ -181,13 +204,18 @@ class StreamDecoder:
             # mode (stream_decoder.py:102-115); otherwise bf16
             self.kv_int8 = bool(kv_int8)
             assert not (self.kv_int8 and attn_ring), "the ring attention kernel reads bf16 caches only"
-            # KV caches: (layer, slot incl. the dummy, head, position, dim); int8 caches carry one fp32 scale per vector
-            kv_dtype = torch.int8 if self.kv_int8 else torch.bfloat16
+            # KV caches: (layer, slot incl. the dummy, head, position, dim); int8 caches carry one fp32 scale per vector,
+            # 4-bit caches hold two dims a byte and carry an fp16 pair (step, lowest) per 64 dims
+            self.kv_int4 = bool(kv_int4)
+            kv_dtype = torch.uint8 if self.kv_int4 else torch.int8 if self.kv_int8 else torch.bfloat16
             for name, cap in (("self", self.seq), ("cross", self.frames)):
                 for part in "kv":
-                    setattr(self, f"{name}_{part}", torch.zeros(L, S + 1, self.h, cap, self.d, device=dev, dtype=kv_dtype))
+                    vecs = (L, S + 1, self.h, cap)
+                    setattr(self, f"{name}_{part}", torch.zeros(*vecs, self.d // 2 if self.kv_int4 else self.d, device=dev,
+                                                                dtype=kv_dtype))
                     setattr(self, f"{name}_{part}s",
-                            torch.ones(L, S + 1, self.h, cap, device=dev) if self.kv_int8 else None)
+                            torch.zeros(*vecs, self.d // 64, 2, device=dev, dtype=torch.float16) if self.kv_int4 else
+                            torch.ones(*vecs, device=dev) if self.kv_int8 else None)
             # slot state, one entry per slot and one for the dummy; names, types and initial values are those of the
             # reference's StreamDecoder (kernels/stream_decoder.py:116-131), which is what its callers read
             i32 = dict(device=dev, dtype=torch.int32)
@@ -204,8 +232,12 @@ class StreamDecoder:
             self._rec_ints = nv.lib().b200dec_admit_record_ints(max_prompt)
             self._admit_cap = max(bm, 16)
             self.admit_buf = torch.zeros(self._admit_cap * self._rec_ints, **i32)
-            self._ring = [(torch.zeros(self._admit_cap * self._rec_ints, dtype=torch.int32).pin_memory(),
-                           torch.cuda.Event()) for _ in range(8)]
+            self.logit_rules, self.max_bias = bool(logit_rules), int(max_bias)
+            words = (self.vocab + 31) // 32
+            # per slot, the table each request brings: slot, three penalties, bias count, mask switch, biases; and the mask's words
+            self._rule_ints = 6 + 2 * self.max_bias + words if self.logit_rules else 0
+            ints = self._admit_cap * max(self._rec_ints, self._rule_ints)
+            self._ring = [(torch.zeros(ints, dtype=torch.int32).pin_memory(), torch.cuda.Event()) for _ in range(8)]
             self._ring_at = 0
             adt = torch.float16 if self.a_kind == nv.A_F16 else torch.float32
             f32 = dict(device=dev, dtype=torch.float32)
@@ -228,7 +260,16 @@ class StreamDecoder:
             # the step's rows ranked by length (self / cross), rebuilt by every step for the paired and span attention kernels
             self.sched_self = torch.zeros(bm, 4, **i32)
             self.sched_cross = torch.zeros(bm, 4, **i32)
-            self.logits = torch.zeros(bm, self.vocab, **f32) if record else None
+            self.logits = torch.zeros(bm, self.vocab, **f32) if record or self.logit_rules else None
+            if self.logit_rules:
+                self.rule_params = torch.zeros(S + 1, 4, **f32)  # repetition, presence, frequency
+                self.rule_bias_ids = torch.zeros(S + 1, self.max_bias, **i32)
+                self.rule_bias = torch.zeros(S + 1, self.max_bias, **f32)
+                self.rule_bias_n = torch.zeros(S + 1, **i32)
+                self.rule_mask = torch.zeros(S + 1, words, **i32)
+                self.rule_mask_on = torch.zeros(S + 1, device=dev, dtype=torch.uint8)
+                self.rule_best, self.rule_token = torch.zeros(bm, **f32), torch.zeros(bm, **i32)
+                self._rule_buf = torch.zeros(self._admit_cap, self._rule_ints, **i32)
             self.argmax = torch.zeros(S + 1, device=dev, dtype=torch.long) if record else None
             # host side: the end flags after each step (pinned, written by the step itself)
             self.flags = torch.ones(S + 1, dtype=torch.uint8).pin_memory()
@@ -256,6 +297,7 @@ class StreamDecoder:
         self.embed = dec.embed_tokens.weight.detach().to(torch.bfloat16).contiguous()
         self.pos_table = dec.pos_emb.weight.detach().to(torch.bfloat16).contiguous()
         ln = lambda m: (_fp32(m.weight), _fp32(m.bias), float(m.eps))  # noqa: E731
+        prefill = _PrefillWeightInt8 if self.prefill_int8 else _PrefillWeight
         self.emb_ln, self.final_ln = ln(dec.embedding_layernorm), ln(dec.norm)
         self.layers = [_Layer(layer, kind, ffn_kind, self.a_kind, bm, keep_reference, umma, self._small_rows)
                        for layer in dec.layers]
@@ -266,9 +308,9 @@ class StreamDecoder:
                                 a_kind=self.head_a_kind, ln=self.final_ln[:2], max_rows=bm)
         # prefill: cross K/V of all layers as one (L * 2 * d, d) matrix behind the encoder projection; these run once
         # per request, not in the step, and keep bf16 weights in every mode, as the reference does
-        # (kernels/stream_decoder.py:91-94, 232)
-        self.proj = _PrefillWeight(_fp32(dec.proj.weight), _fp32(dec.proj.bias))
-        self.cross = _PrefillWeight(
+        # (kernels/stream_decoder.py:91-94, 232), unless prefill_int8 asks for 8 bits
+        self.proj = prefill(_fp32(dec.proj.weight), _fp32(dec.proj.bias))
+        self.cross = prefill(
             torch.cat([_fp32(w) for layer in dec.layers
                        for w in (layer.encoder_attn.k_proj.weight, layer.encoder_attn.v_proj.weight)]),
             torch.cat([_fp32(b) for layer in dec.layers
@@ -299,7 +341,9 @@ class StreamDecoder:
             self.layers.append(ly)
         self.head = packed("head")
         for name in ("proj", "cross"):
-            w = object.__new__(_PrefillWeight)
+            w = object.__new__(_PrefillWeightInt8 if self.prefill_int8 else _PrefillWeight)
+            if self.prefill_int8:
+                w.scale = t[f"prefill.{name}.scale"]
             w.image, w.bias = nv.image(t[f"prefill.{name}.image"].numel(), self.device), t[f"prefill.{name}.bias"]
             w.image.copy_(t[f"prefill.{name}.image"])
             w.n, w.k = manifest["prefill"][name]
@@ -346,7 +390,8 @@ class StreamDecoder:
             raise ValueError("umma_above_rows is a packing option: it comes from the file")
         self = cls(shim, int8=po["int8"], fp16_weights=po.get("fp16_weights", False), ffn_sparse=po["ffn_sparse"],
                    head_split=po["head_split"], umma_above_rows=po.get("small_rows", 0),
-                   head_umma=po["head_umma"], proj_umma=po["proj_umma"] or False, _packed=(man, blob["tensors"]), **kw)
+                   head_umma=po["head_umma"], proj_umma=po["proj_umma"] or False,
+                   prefill_int8=po.get("prefill_int8", False), _packed=(man, blob["tensors"]), **kw)
         if self.weights_digest() != man["sha256"]:
             raise ValueError(f"{path}: the packed weights do not match the manifest's SHA-256")
         return self
@@ -378,7 +423,7 @@ class StreamDecoder:
                     setattr(s, name, ((ly.small.get(name) if small else None) or getattr(ly, name)).struct())
                 s.self_k, s.self_v = nv.ptr(self.self_k[i]), nv.ptr(self.self_v[i])
                 s.cross_k, s.cross_v = nv.ptr(self.cross_k[i]), nv.ptr(self.cross_v[i])
-                if self.kv_int8:
+                if self.kv_int8 or self.kv_int4:
                     s.self_ks, s.self_vs = nv.ptr(self.self_ks[i]), nv.ptr(self.self_vs[i])
                     s.cross_ks, s.cross_vs = nv.ptr(self.cross_ks[i]), nv.ptr(self.cross_vs[i])
             return structs
@@ -403,9 +448,18 @@ class StreamDecoder:
         # pinned host memory is addressable from the device: a row that ends sets its byte of `flags` from the pick
         # kernel (admit() clears it on the host, as the reference does)
         p.flags_host = self.flags.data_ptr()
+        p.kv_int4 = int(self.kv_int4)
+        if self.logit_rules:
+            self._rules = nv.Rules(*(nv.ptr(t) for t in (self.rule_params, self.out, self.pos, self.plen, self.rule_bias_ids,
+                                                         self.rule_bias, self.rule_bias_n, self.rule_mask, self.rule_mask_on)),
+                                   self.out.shape[1], self.max_bias)
+            p.rules, p.rule_best, p.rule_token = C.pointer(self._rules), nv.ptr(self.rule_best), nv.ptr(self.rule_token)
         self.plan = p
         # what every fill_cross hands to its two products
-        weight = lambda w: (w.k, nv.ptr(w.image), nv.ptr(w.bias), w.n)  # noqa: E731
+        def weight(w):
+            if self.prefill_int8:
+                return w.k, nv.ptr(w.image), nv.ptr(w.scale), nv.ptr(w.bias), w.n
+            return w.k, nv.ptr(w.image), nv.ptr(w.bias), w.n
         self._prefill_args = (nv.ptr(self.status), weight(self.proj), weight(self.cross),
                               (*(nv.ptr(t) for t in (self.cross_k, self.cross_v, self.cross_ks, self.cross_vs)), L,
                                self.slots + 1, self.h, self.d, self.frames))
@@ -529,6 +583,10 @@ class StreamDecoder:
             for t, v in ((self.finished, 1), (self.pos, 0), (self.cross_len, 1), (self.active, self.dummy),
                          (self.status, 0), (self.attn_count, 0), (self.n_active, 0)):
                 t.fill_(v)
+            if self.logit_rules:  # no slot asks for anything
+                for t in (self.rule_params, self.rule_bias_n, self.rule_mask_on):
+                    t.fill_(0)
+                self.rule_params[:, 0] = 1.0
         self.flags.fill_(1)  # the host's copy (the steps write it through; nothing is in flight at a reset)
 
     def check_status(self) -> None:
@@ -541,7 +599,8 @@ class StreamDecoder:
                                       ("out-of-range position", nv.ST_POS_RANGE),
                                       ("out-of-range frame count", nv.ST_FRAMES_RANGE),
                                       ("out-of-range slot", nv.ST_SLOT_RANGE),
-                                      ("a bounded wait inside a kernel ran out", nv.ST_TIMEOUT)) if st & bit]
+                                      ("a bounded wait inside a kernel ran out", nv.ST_TIMEOUT),
+                                      ("a row whose rules left no token (0 was taken)", nv.ST_NO_TOKEN)) if st & bit]
             raise nv.NativeError("decoder kernels reported: " + ", ".join(names))
 
     # ---- host side -----------------------------------------------------------------------------------------------
@@ -584,15 +643,15 @@ class StreamDecoder:
         if m == 0:
             return
         lib, cur = nv.lib(), torch.cuda.current_stream()
+        if self.prefill_int8:
+            return self._fill_cross_int8(hidden, lengths, slots)
         x, high = hidden.contiguous(), 0
         if hidden.dtype == torch.bfloat16 and x.is_cuda:
             high = nv.PREFILL_HIGH_ROWS
             x = x if x.data_ptr() % 16 == 0 else x.clone()
         else:
             x = x.float()
-        pieces = np.zeros((len(slots), 4), np.int32)
-        pieces[1:, 0] = np.cumsum(lengths[:-1])
-        pieces[:, 1], pieces[:, 2] = lengths, slots
+        pieces = self._pieces(lengths, slots)
         # the two operand images, on a 1 KB boundary, and the table of pieces
         n0, n1 = lib.b200dec_prefill_rows_bytes(m, self.proj.k), lib.b200dec_prefill_rows_bytes(m, self.proj.n)
         work = torch.empty(1024 + n0 + n1 + pieces.nbytes, dtype=torch.uint8, device=self.device)
@@ -600,23 +659,70 @@ class StreamDecoder:
         a0 = work.data_ptr() + pad
         a1 = a0 + n0
         table = work[pad + n0 + n1:pad + n0 + n1 + pieces.nbytes].view(torch.int32)
-        if pieces.size <= self._ring[0][0].numel():
-            self._stage_here(pieces, table, cur)
-        else:
-            table.copy_(torch.from_numpy(pieces.reshape(-1)))
+        self._stage_pieces(pieces, table, cur)
         s, (status, first, second, caches) = cur.cuda_stream, self._prefill_args
         pack = lib.b200dec_prefill_pack_rows_bf16 if high else lib.b200dec_prefill_pack_rows
         nv.check(pack(nv.ptr(x), m, self.proj.k, x.shape[1], a0, s))
         nv.check(lib.b200dec_prefill_gemm(a0, m, *first, 0 | high, a1, None, 0, None, None, None, None, 0, 0, 0, 0, 0,
                                           status, s))
-        nv.check(lib.b200dec_prefill_gemm(a1, m, *second, 2 if self.kv_int8 else 1, None, a1 + n1, len(slots), *caches,
+        nv.check(lib.b200dec_prefill_gemm(a1, m, *second, self._cache_mode(), None, a1 + n1, len(slots), *caches,
                                           status, s))
         hidden.record_stream(cur)  # the others come from this stream's pool
 
-    def admit(self, slots: list[int], prompts: list, frames: list[int], max_new: list[int] | None = None) -> None:
+    def _cache_mode(self) -> int:
+        return 3 if self.kv_int4 else 2 if self.kv_int8 else 1
+
+    @staticmethod
+    def _pieces(lengths: list[int], slots: list[int]) -> np.ndarray:
+        pieces = np.zeros((len(slots), 4), np.int32)
+        pieces[1:, 0] = np.cumsum(lengths[:-1])
+        pieces[:, 1], pieces[:, 2] = lengths, slots
+        return pieces
+
+    def _stage_pieces(self, pieces: np.ndarray, table: torch.Tensor, stream: torch.cuda.Stream) -> None:
+        if pieces.size <= self._ring[0][0].numel():
+            self._stage_here(pieces, table, stream)
+        else:
+            table.copy_(torch.from_numpy(pieces.reshape(-1)))
+
+    def _fill_cross_int8(self, hidden: torch.Tensor, lengths: list[int], slots: list[int]) -> None:
+        """fill_cross with both products in 8-bit integers: the frames quantised as they come, then the fp32 rows between."""
+        lib, cur, m = nv.lib(), torch.cuda.current_stream(), int(hidden.shape[0])
+        kinds = {torch.float32: nv.T_F32, torch.float16: nv.T_F16, torch.bfloat16: nv.T_BF16}
+        x = hidden.to(self.device)
+        x = x if x.dtype in kinds else x.float()
+        x = x if x.stride(1) == 1 and (m == 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+        pieces = self._pieces(lengths, slots)
+        # the two operand images on 1 KB boundaries, their scales, the rows between the products, the table of pieces
+        n0, n1 = lib.b200dec_w8a8_rows_bytes(m, self.proj.k), lib.b200dec_w8a8_rows_bytes(m, self.proj.n)
+        scales, rows = -(-4 * m // 1024) * 1024, 4 * m * self.proj.n
+        work = torch.empty(1024 + n0 + n1 + scales + rows + pieces.nbytes, dtype=torch.uint8, device=self.device)
+        pad = -work.data_ptr() % 1024
+        a0 = work.data_ptr() + pad
+        a1, sc, mid = a0 + n0, a0 + n0 + n1, a0 + n0 + n1 + scales
+        at = pad + n0 + n1 + scales + rows
+        self._stage_pieces(pieces, work[at:at + pieces.nbytes].view(torch.int32), cur)
+        s, (status, first, second, caches) = cur.cuda_stream, self._prefill_args
+        (k0, w0, s0, b0, c0), (k1, w1, s1, b1, c1) = first, second
+        nv.check(lib.b200dec_w8a8_pack_rows(x.data_ptr(), kinds[x.dtype], m, k0, x.stride(0), a0, sc, s))
+        nv.check(lib.b200dec_w8a8_linear(a0, sc, m, k0, w0, s0, b0, c0, nv.ACT_NONE, mid, nv.T_F32, c0, status, s))
+        nv.check(lib.b200dec_w8a8_pack_rows(mid, nv.T_F32, m, k1, k1, a1, sc, s))
+        nv.check(lib.b200dec_w8a8_prefill(a1, sc, m, k1, w1, s1, b1, c1, self._cache_mode(), work.data_ptr() + at, len(slots), *caches,
+                                          status, s))
+        if hidden.is_cuda:
+            hidden.record_stream(cur)  # the others come from this stream's pool
+
+    def admit(self, slots: list[int], prompts: list, frames: list[int], max_new: list[int] | None = None,
+              rules: list[dict | None] | None = None) -> None:
         """Start decoding in `slots`: each gets its prompt (fed token by token as forced choices), its number of
-        encoder frames and its new-token budget (max_new_tokens when not given). On the decoder stream."""
+        encoder frames and its new-token budget (max_new_tokens when not given). On the decoder stream. rules (of a decoder
+        with logit_rules): per request None or a dict of what its tokens are chosen under: "repetition" (> 0; 1: none, over
+        prompt and generated tokens), "presence", "frequency" (of generated tokens), "bias" (token -> what is added to its
+        logit, -inf bans it) and "mask" (see set_mask). Without them a slot is decoded greedily as ever."""
         n = len(slots)
+        if rules is not None and (not self.logit_rules or len(rules) != n):
+            raise ValueError("admit: one set of rules (or None) per slot, in a decoder made with logit_rules=True")
+        tables = self._rule_tables(slots, rules or [None] * n) if self.logit_rules else None
         budgets = list(max_new) if max_new else [self.max_new_tokens] * n
         if not (len(prompts) == len(frames) == len(budgets) == n):
             raise ValueError("admit: one prompt, frame count and budget per slot")
@@ -631,6 +737,8 @@ class StreamDecoder:
             rec[i, :4] = (s, p.size, m, f)
             rec[i, 4:4 + p.size] = p
         torch.cuda.nvtx.range_push("b200dec.admit")
+        if tables is not None:
+            self._put_rules(tables)
         for i0 in range(0, n, self._admit_cap):  # more requests than the staging buffer holds: several launches
             part = rec[i0:i0 + self._admit_cap]
             self._stage(part, self.admit_buf)
@@ -639,6 +747,81 @@ class StreamDecoder:
                                             self.stream.cuda_stream))
         self.flags.numpy()[list(slots)] = 0
         torch.cuda.nvtx.range_pop()
+
+    def _mask_words(self, mask) -> np.ndarray:
+        """A mask over the vocabulary (booleans, True = allowed) or its ready words (32 tokens each, lowest bit first)."""
+        m = mask.detach().cpu().numpy() if isinstance(mask, torch.Tensor) else np.asarray(mask)
+        words = (self.vocab + 31) // 32
+        if m.shape == (self.vocab,) and m.dtype == np.bool_:
+            return np.packbits(np.pad(m, (0, 32 * words - self.vocab)), bitorder="little").view(np.int32)
+        if m.shape == (words,) and m.dtype in (np.int32, np.uint32):
+            return m.view(np.int32)
+        raise ValueError(f"mask: {self.vocab} booleans or {words} 32-bit words")
+
+    def _rule_tables(self, slots: list[int], rules: list[dict | None]) -> np.ndarray:
+        """One record per request: slot, penalties, bias count, mask switch, bias ids, bias values, mask words."""
+        rec = np.zeros((len(slots), self._rule_ints), np.int32)
+        f, nb = rec.view(np.float32), self.max_bias
+        rec[:, 0], f[:, 1] = slots, 1.0
+        for i, r in enumerate(rules):
+            r = r or {}
+            unknown = set(r) - {"repetition", "presence", "frequency", "bias", "mask"}
+            bias = dict(r.get("bias") or {})
+            pens = [float(r.get(k, d)) for k, d in (("repetition", 1.0), ("presence", 0.0), ("frequency", 0.0))]
+            if unknown or len(bias) > nb or not np.all(np.isfinite(pens)) or pens[0] <= 0:
+                raise ValueError(f"admit: rules {sorted(unknown) or pens} with {len(bias)} biases (at most {nb}; repetition > 0)")
+            ids, vals = [int(k) for k in bias], [float(v) for v in bias.values()]
+            if any(not 0 <= k < self.vocab for k in ids) or any(np.isnan(v) for v in vals):
+                raise ValueError("admit: a bias for a token outside the vocabulary, or that is no number")
+            f[i, 1:4], rec[i, 4] = pens, len(bias)
+            rec[i, 6:6 + len(ids)], f[i, 6 + nb:6 + nb + len(ids)] = ids, vals
+            if r.get("mask") is not None:
+                rec[i, 5], rec[i, 6 + 2 * nb:] = 1, self._mask_words(r["mask"])
+        return rec
+
+    @staticmethod
+    def _last_of_each(rec: np.ndarray) -> np.ndarray:
+        """A slot named twice keeps its last record (the copies into the tables have no order of their own)."""
+        return rec[sorted({int(s): i for i, s in enumerate(rec[:, 0])}.values())]
+
+    def _put_rules(self, rec: np.ndarray) -> None:
+        nb, rec = self.max_bias, self._last_of_each(rec)
+        for i0 in range(0, len(rec), self._admit_cap):
+            part = rec[i0:i0 + self._admit_cap]
+            with torch.cuda.stream(self.stream):
+                self._stage_here(part, self._rule_buf.view(-1), self.stream)
+                t = self._rule_buf[:len(part)]
+                at, f = t[:, 0].long(), t.view(torch.float32)
+                self.rule_params[:, :3].index_copy_(0, at, f[:, 1:4])
+                self.rule_bias_n.index_copy_(0, at, t[:, 4])
+                self.rule_bias_ids.index_copy_(0, at, t[:, 6:6 + nb])
+                self.rule_bias.index_copy_(0, at, f[:, 6 + nb:6 + 2 * nb])
+                self.rule_mask.index_copy_(0, at, t[:, 6 + 2 * nb:])
+                self.rule_mask_on.index_copy_(0, at, t[:, 5].to(torch.uint8))
+
+    def set_mask(self, slots: list[int], masks: list) -> None:
+        """What the next steps of these slots may choose: per slot None (everything), booleans over the vocabulary (True =
+        allowed), or the mask's 32-bit words (bit v % 32 of word v / 32); holds until it is set again or the slot admits
+        another request. A grammar sets it between steps. On the decoder stream, so it counts from the next step
+        launched. A mask that allows nothing makes the choice token 0 and is reported by check_status."""
+        if not self.logit_rules or len(masks) != len(slots) or not all(0 <= s < self.slots for s in slots):
+            raise ValueError(f"set_mask: one mask per slot (0..{self.slots - 1}), in a decoder made with logit_rules=True")
+        words = (self.vocab + 31) // 32
+        rec = np.zeros((len(slots), 2 + words), np.int32)
+        for i, (s, m) in enumerate(zip(slots, masks)):
+            rec[i, :2] = s, m is not None
+            if m is not None:
+                rec[i, 2:] = self._mask_words(m)
+        rec = self._last_of_each(rec)
+        for i0 in range(0, len(rec), self._admit_cap):
+            part = rec[i0:i0 + self._admit_cap]
+            with torch.cuda.stream(self.stream):
+                flat = self._rule_buf.view(-1)
+                self._stage_here(part, flat, self.stream)
+                t = flat[:part.size].view(part.shape)
+                at = t[:, 0].long()
+                self.rule_mask.index_copy_(0, at, t[:, 2:])
+                self.rule_mask_on.index_copy_(0, at, t[:, 1].to(torch.uint8))
 
     def set_active(self, slots: list[int]) -> int:
         """The rows of the next steps = these slots, padded with the dummy slot to a bucket; returns the bucket."""
@@ -701,6 +884,8 @@ class StreamDecoder:
                 out[f"layer{i}.ln{j + 1}.w"], out[f"layer{i}.ln{j + 1}.b"] = w, b
         for name, p in (("prefill.proj", self.proj), ("prefill.cross", self.cross)):
             out[name + ".image"], out[name + ".bias"] = p.image, p.bias
+            if self.prefill_int8:
+                out[name + ".scale"] = p.scale
         return out
 
     def weights_digest(self) -> str:
@@ -724,6 +909,7 @@ class StreamDecoder:
         pad = (rows or len(positions)) - len(positions)
         kv = sum((int(p) + 1) + int(t) for p, t in zip(positions, frames)) + pad * 2
         n = len(positions) + pad
-        # bytes per cached or appended vector element: 2 (bf16), or 1 + 4 / D (int8 and its share of the vector's scale)
-        b_kv = 1 + 4 / self.d if self.kv_int8 else 2
+        # bytes per cached or appended vector element: 2 (bf16), 1 + 4 / D (int8 and its share of the vector's scale), or
+        # 1/2 + 4 / 64 (4 bits and its share of the group's pair)
+        b_kv = 0.5 + 4 / 64 if self.kv_int4 else 1 + 4 / self.d if self.kv_int8 else 2
         return int(self.weight_bytes + L * 2 * d * b_kv * kv + n * L * 2 * d * b_kv + n * 2 * d * 2)

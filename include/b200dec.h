@@ -77,11 +77,27 @@ typedef struct b200dec_layer {
   void* self_v;
   const void* cross_k; /* bf16 or int8 (slots + 1, H, frames, D) */
   const void* cross_v;
-  float* self_ks;      /* kv_int8: one fp32 scale per cached vector, (slots + 1, H, seq); else NULL */
+  float* self_ks;      /* kv_int8: one fp32 scale per cached vector, (slots + 1, H, seq); else NULL (kv_int4: the pairs) */
   float* self_vs;
   float* cross_ks;     /* (slots + 1, H, frames) */
   float* cross_vs;
 } b200dec_layer;
+
+/* What a slot's request asks of the choice of its tokens (b200dec_logit_rules); every table has slots + 1 rows, in device memory.
+ * No counterpart in the reference. */
+typedef struct b200dec_rules {
+  const float* params;     /* (slots + 1, 4), 16-byte aligned: repetition penalty (> 0; 1: none), presence penalty, frequency
+                              penalty (0: none), unused */
+  const int64_t* history;  /* (slots + 1, hist_cols): the slot's tokens; ids outside the vocabulary count for nothing */
+  const int32_t* last;     /* (slots + 1): history[0 .. last] counts (-1: none), last < hist_cols */
+  const int32_t* plen;     /* (slots + 1): history[plen .. last] are generated, what is before them is the prompt */
+  const int32_t* bias_ids; /* NULL (with the next two), or (slots + 1, max_bias) token ids, */
+  const float* bias;       /* what is added to their logits (-INFINITY bans a token; one listed twice gets both), */
+  const int32_t* bias_n;   /* and how many of a slot's entries count */
+  const uint32_t* mask;    /* NULL, or (slots + 1, (vocab + 31) / 32): bit v % 32 of word v / 32 set = token v is allowed */
+  const uint8_t* mask_on;  /* NULL: every slot has a mask; else (slots + 1), 0: the slot's mask is not looked at */
+  int32_t hist_cols, max_bias;  /* max_bias <= 1024 */
+} b200dec_rules;
 
 /* Everything one decoding step touches. Replaces the argument lists of StreamDecoder._step
  * (kernels/stream_decoder.py:176-199). */
@@ -151,6 +167,14 @@ typedef struct b200dec_plan {
    * kernel's CTAs wait for one another, so the caller keeps fused steps of different streams from running at the same
    * time on one device. withhold bit 2 (tests only): one CTA leaves out one result, so the waits for it run out. */
   void* fused_ws[16];
+  /* kv_int4 != 0: 4-bit caches (see b200dec_attention_q4); the layers' caches hold codes, self_ks .. cross_vs their fp16 pairs.
+   * rules: NULL, or the rules the choice goes by (a host struct of device tables): the step then writes its logits, b200dec_logit_rules
+   * takes them into rule_best / rule_token (max rows each), and the pick chooses from those; `logits` must be there and keeps
+   * the logits before the rules. Steps with either are not fused. */
+  int32_t kv_int4, _pad2;
+  const b200dec_rules* rules;
+  float* rule_best;
+  int32_t* rule_token;
 } b200dec_plan;
 
 const char* b200dec_last_error(void);
@@ -368,21 +392,7 @@ int b200dec_scatter_kv_q4(const float* kv, const int32_t* slot_of, const int32_t
 int b200dec_gather_kv_q4(float* kv, const int32_t* slot_of, const int32_t* frame_of, const void* ck, const void* cv,
                          const void* ck_pairs, const void* cv_pairs, int nrows, int layers, int slots_plus_1, int heads,
                          int head_dim, int frames, void* stream);
-/* ---- rules on the logits ----------------------------------------------------------------------------------------------
- * What a slot's request asks of the choice of its tokens; every table has slots + 1 rows, in device memory. */
-typedef struct b200dec_rules {
-  const float* params;     /* (slots + 1, 4), 16-byte aligned: repetition penalty (> 0; 1: none), presence penalty, frequency
-                              penalty (0: none), unused */
-  const int64_t* history;  /* (slots + 1, hist_cols): the slot's tokens; ids outside the vocabulary count for nothing */
-  const int32_t* last;     /* (slots + 1): history[0 .. last] counts (-1: none), last < hist_cols */
-  const int32_t* plen;     /* (slots + 1): history[plen .. last] are generated, what is before them is the prompt */
-  const int32_t* bias_ids; /* NULL (with the next two), or (slots + 1, max_bias) token ids, */
-  const float* bias;       /* what is added to their logits (-INFINITY bans a token; one listed twice gets both), */
-  const int32_t* bias_n;   /* and how many of a slot's entries count */
-  const uint32_t* mask;    /* NULL, or (slots + 1, (vocab + 31) / 32): bit v % 32 of word v / 32 set = token v is allowed */
-  const uint8_t* mask_on;  /* NULL: every slot has a mask; else (slots + 1), 0: the slot's mask is not looked at */
-  int32_t hist_cols, max_bias;  /* max_bias <= 1024 */
-} b200dec_rules;
+/* ---- rules on the logits (b200dec_rules above) -------------------------------------------------------------------------- */
 /* The greedy choice of every row under its slot's rules, slot = active[r]. With x a token's logit (fp32, fp16 or bf16 by
  * kind, row r at logits + r * ldl): x = x > 0 ? x / repetition : x * repetition where the token is in the slot's history,
  * then x - frequency * (times generated) - presence where it was generated, then x + its biases, then -INFINITY where the
