@@ -460,10 +460,7 @@ __global__ void __launch_bounds__(NTHREADS) attention_q4_kernel(const Q4Args p) 
 
 template <int D, bool SELF, int WPI>
 cudaError_t launch_wpi(int splits, int rows, cudaStream_t st, int pdl, const Q4Args& p) {
-  if (Ring<D>::BYTES > 32 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(attention_q4_kernel<D, SELF, WPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<D>::BYTES);
-    if (e != cudaSuccess) return e;
-  }
+  static_assert(Ring<D>::BYTES <= 40 * 1024, "with the static arrays below 48 KB: no attribute to set");
   const dim3 grid(splits, (p.H + WARPS / WPI - 1) / (WARPS / WPI), rows);
   return launch_kernel(attention_q4_kernel<D, SELF, WPI>, grid, dim3(NTHREADS), Ring<D>::BYTES, st, 0, pdl, p);
 }

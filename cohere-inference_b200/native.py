@@ -198,7 +198,9 @@ def image(n: int, device) -> torch.Tensor:
 
 
 def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
-    return (stream or torch.cuda.current_stream()).cuda_stream
+    """The given stream's handle, or the current one's of the current device (asked for as a number: a Stream object for it
+    takes 3 us to make, a third of a small call)."""
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def norm(weight: torch.Tensor, bias: torch.Tensor, eps: float) -> Norm:

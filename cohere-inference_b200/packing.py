@@ -230,39 +230,49 @@ class W8A8Linear:
             q = q.contiguous()
             nv.check(lib.b200dec_w8a8_tile_weight(nv.ptr(q), self.n, self.k, nv.ptr(self.image), nv.stream_ptr()))
             torch.cuda.current_stream().synchronize()  # any stream may use the image from now on
+        self._weight = nv.ptr(self.image), nv.ptr(self.scale), nv.ptr(self.bias), self.n, self.act
+        self._status = nv.ptr(self.status)
 
     @classmethod
     def from_weight(cls, w: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None) -> "W8A8Linear":
         """The weight (n, k) quantised by quantize_rows."""
         return cls(*quantize_rows(w), bias, act)
 
-    def _rows(self, x: torch.Tensor) -> tuple[int, torch.Tensor, int, int]:
-        """Checks x (m, k), quantises its rows on the current stream: m, the work buffer, the image's and the scales' address."""
-        if not (x.device == self.device and x.dim() == 2 and x.shape[1] == self.k and x.dtype in self.KINDS):
-            raise ValueError(f"W8A8Linear: rows of {self.k} fp32, fp16 or bf16 values on {self.device}")
-        if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < self.k):
-            x = x.contiguous()
-        m, lib = int(x.shape[0]), nv.lib()
-        size = lib.b200dec_w8a8_rows_bytes(m, self.k)
-        work = torch.empty(1024 + size + 4 * m, dtype=torch.uint8, device=self.device)
-        image = work.data_ptr() + -work.data_ptr() % 1024
-        if m:
-            nv.check(lib.b200dec_w8a8_pack_rows(x.data_ptr(), self.KINDS[x.dtype], m, self.k, x.stride(0), image, image + size,
-                                                nv.stream_ptr()))
-        return m, work, image, image + size
-
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
         """x (m, k) fp32, fp16 or bf16, rows any distance apart -> (m, n) of x's type (or dtype, or into out, rows any distance
         apart)."""
+        dev, kinds = self.device, self.KINDS
+        x_kind = kinds.get(x.dtype)
+        if x_kind is None or x.device != dev or x.dim() != 2 or x.shape[1] != self.k:
+            raise ValueError(f"W8A8Linear: rows of {self.k} fp32, fp16 or bf16 values on {dev}")
+        m, (ldx, dx) = x.shape[0], x.stride()
+        if dx != 1 or (m > 1 and ldx < self.k):
+            x = x.contiguous()
+            ldx = self.k
         if out is None:
-            out = torch.empty(x.shape[0], self.n, dtype=dtype or x.dtype, device=self.device)
-        if not (out.device == self.device and out.shape == (x.shape[0], self.n) and out.dtype in self.KINDS and out.stride(1) == 1
-                and (out.shape[0] <= 1 or out.stride(0) >= self.n) and dtype in (None, out.dtype)):
-            raise ValueError(f"W8A8Linear: out must be ({x.shape[0]}, {self.n}) fp32, fp16 or bf16 with dense rows on {self.device}")
-        with torch.cuda.device(self.device):
-            m, work, image, scales = self._rows(x)
-            if m:
-                nv.check(nv.lib().b200dec_w8a8_linear(image, scales, m, self.k, nv.ptr(self.image), nv.ptr(self.scale),
-                                                      nv.ptr(self.bias), self.n, self.act, out.data_ptr(), self.KINDS[out.dtype],
-                                                      out.stride(0), nv.ptr(self.status), nv.stream_ptr()))
+            out = torch.empty(m, self.n, dtype=dtype or x.dtype, device=dev)
+        kind = kinds.get(out.dtype)
+        if kind is None or out.device != dev or out.shape != (m, self.n) or dtype not in (None, out.dtype):
+            raise ValueError(f"W8A8Linear: out must be ({m}, {self.n}) fp32, fp16 or bf16 on {dev}")
+        ldo, do = out.stride()
+        if m == 0:
+            return out
+        if (do != 1 and self.n > 1) or (m > 1 and ldo < self.n):
+            raise ValueError("W8A8Linear: out's rows must be dense and apart")
+        if torch.cuda.current_device() != dev.index:
+            with torch.cuda.device(dev):
+                return self._run(x, x_kind, m, ldx, out, kind, ldo)
+        return self._run(x, x_kind, m, ldx, out, kind, ldo)
+
+    def _run(self, x, x_kind, m, ldx, out, kind, ldo) -> torch.Tensor:
+        lib, k = nv.lib(), self.k
+        size = -(-m // 128) * 128 * (-(-k // 128) * 128)  # b200dec_w8a8_rows_bytes
+        work = torch.empty(1024 + size + 4 * m, dtype=torch.uint8, device=self.device)  # the rows' image, their scales
+        image = work.data_ptr()
+        image += -image % 1024
+        stream = nv.stream_ptr()
+        rc = lib.b200dec_w8a8_pack_rows(x.data_ptr(), x_kind, m, k, ldx, image, image + size, stream) or lib.b200dec_w8a8_linear(
+            image, image + size, m, k, *self._weight, out.data_ptr(), kind, ldo, self._status, stream)
+        if rc:
+            nv.check(rc)
         return out
