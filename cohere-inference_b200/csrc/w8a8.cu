@@ -377,7 +377,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) w8a8_kernel(const W8Args p) {
 // Rows -> 8-bit integers with one scale a row: s = max(max |x|, 1e-12) / 127, q = rint(x / s), both as if the quotients were
 // exact: the product with the reciprocal is off by a few 2^-23 of it, so only its rounding beside a half can be wrong, and
 // the remainder x - q s (exact: a multiple of ulp(s) / 2 below 2^24 of them) decides there. A row with an infinity or NaN gets
-// scale NaN: its results are NaN. One warp a row, which passes over it twice (the second time out of L1 and L2).
+// scale NaN: its results are NaN. One warp a row; rows of up to 1024 values stay in registers between the largest magnitude
+// and the codes, longer ones are read again.
 template <class X>
 DEVI float row_value(X x) {
   if constexpr (std::is_same<X, float>::value) return x;
@@ -385,22 +386,24 @@ DEVI float row_value(X x) {
   else return __bfloat162float(x);
 }
 
-// values c .. c + 15 of a row of k, zeros past its end
-template <class X, bool WIDE>
-DEVI void load_16(const X* row, int c, int k, float (&f)[16]) {
-  if (WIDE && c + 16 <= k) {
-    constexpr int PER = 16 / (int)sizeof(X);
+// This lane's 16 of the 512 values from c on of a row of k, zeros past its end: loads of A bytes, neighbouring lanes side by side.
+template <class X, int A>
+DEVI void load_16(const X* row, int c, int k, int lane, float (&f)[16]) {
+  constexpr int V = A / (int)sizeof(X);
 #pragma unroll
-    for (int i = 0; i < 16 / PER; ++i) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
-      X x[PER];
-      memcpy(x, &w, 16);
+  for (int j = 0; j < 16 / V; ++j) {
+    const int at = c + (lane + 32 * j) * V;
+    if (V > 1 && at + V <= k) {
+      X x[V];
+      if constexpr (A == 16) *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(row + at));
+      else if constexpr (A == 8) *reinterpret_cast<uint2*>(x) = __ldg(reinterpret_cast<const uint2*>(row + at));
+      else *reinterpret_cast<uint32_t*>(x) = __ldg(reinterpret_cast<const uint32_t*>(row + at));
 #pragma unroll
-      for (int j = 0; j < PER; ++j) f[i * PER + j] = row_value(x[j]);
+      for (int i = 0; i < V; ++i) f[j * V + i] = row_value(x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[j * V + i] = at + i < k ? row_value(row[at + i]) : 0.f;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = c + i < k ? row_value(row[c + i]) : 0.f;
   }
 }
 
@@ -413,20 +416,46 @@ DEVI int code8(float x, float s, float inv) {
   return (int)fminf(fmaxf(c, -127.f), 127.f);
 }
 
-template <class X, bool WIDE>
+// The same for 16 values: adding 1.5 * 2^23 rounds the product, whose low byte is the code then (two's complement); only where one
+// of them is within 2^-15 of a half, four times what the reciprocal can be off, does the remainder decide.
+DEVI void codes16(const float (&x)[16], float s, float inv, uint8_t (&q)[16]) {
+  constexpr float MAGIC = 12582912.f;
+  float near = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float t = __fmaf_rn(x[i], inv, MAGIC);
+    near = fmaxf(near, fabsf(__fmaf_rn(x[i], inv, MAGIC - t)));
+    q[i] = (uint8_t)__float_as_uint(t);
+  }
+  if (near > 0.5f - 3.0517578e-05f) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q[i] = (uint8_t)code8(x[i], s, inv);
+  }
+}
+
+template <class X, int A>
 __global__ void __launch_bounds__(256) pack_rows_i8_kernel(const X* __restrict__ x, int m, int k, int64_t ldx,
                                                            unsigned char* __restrict__ image, float* __restrict__ scale) {
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  constexpr int V = A / (int)sizeof(X), KEPT = 2;  // 512 values each
+  __shared__ __align__(16) uint8_t s_codes[8][512];
+  const int warp = threadIdx.x >> 5, row = blockIdx.x * 8 + warp, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
   if (row >= m) return;  // the rows that fill the last tile up are never stored: whatever the image holds there does no harm
   const X* src = x + row * ldx;
   uint32_t top = 0;  // largest magnitude by its bits, so that a NaN is the largest
-  for (int c = lane * 16; c < k; c += 512) {
-    float f[16];
-    load_16<X, WIDE>(src, c, k, f);
+  float kept[KEPT][16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+  for (int i = 0; i < KEPT; ++i) load_16<X, A>(src, 512 * i, k, lane, kept[i]);
+#pragma unroll
+  for (int i = 0; i < KEPT; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(kept[i][j]) & 0x7fffffffu);
+  for (int c = 512 * KEPT; c < k; c += 512) {
+    float f[16];
+    load_16<X, A>(src, c, k, lane, f);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
   }
   top = __reduce_max_sync(0xffffffffu, top);
   const float s = top < 0x7f800000u ? __fdiv_rn(fmaxf(__uint_as_float(top), 1e-12f), 127.f) : __uint_as_float(0x7fffffffu);
@@ -434,13 +463,38 @@ __global__ void __launch_bounds__(256) pack_rows_i8_kernel(const X* __restrict__
   if (lane == 0) scale[row] = s;
   const int kp = (k + 127) / 128 * 128;
   unsigned char* tile = image + (size_t)(row / BM) * (kp / 128) * A_STAGE;
-  for (int c = lane * 16; c < kp; c += 512) {
-    float f[16];
-    load_16<X, WIDE>(src, c, k, f);
-    uint32_t w[4] = {0, 0, 0, 0};
+  const auto put = [&](int c, const float (&f)[16]) {  // 512 codes through shared memory into pieces of 16
+    uint8_t* codes = s_codes[warp];
+    __syncwarp();
+    uint8_t q[16];
+    codes16(f, s, inv, q);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i >> 2] |= (uint32_t)(code8(f[i], s, inv) & 0xff) << ((i & 3) * 8);
-    *reinterpret_cast<uint4*>(tile + (size_t)(c / 128) * A_STAGE + swz(row % BM, (c % 128) / 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < 16 / V; ++j) {
+      uint8_t* to = codes + (lane + 32 * j) * V;
+      if constexpr (V >= 4) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+          const uint8_t* b = q + j * V + i;
+          *reinterpret_cast<uint32_t*>(to + i) = b[0] | b[1] << 8 | b[2] << 16 | (uint32_t)b[3] << 24;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = q[j * V + i];
+      }
+    }
+    __syncwarp();
+    const int at = c + 16 * lane;
+    if (at < kp)
+      *reinterpret_cast<uint4*>(tile + (size_t)(at / 128) * A_STAGE + swz(row % BM, (at % 128) / 16)) =
+          *reinterpret_cast<const uint4*>(codes + 16 * lane);
+  };
+#pragma unroll
+  for (int i = 0; i < KEPT; ++i)
+    if (512 * i < kp) put(512 * i, kept[i]);
+  for (int c = 512 * KEPT; c < kp; c += 512) {
+    float f[16];
+    load_16<X, A>(src, c, k, lane, f);
+    put(c, f);
   }
 }
 
@@ -458,12 +512,16 @@ __global__ void tile_weight_i8_kernel(const int8_t* __restrict__ q, int n, int k
       make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The widest loads that the rows' addresses and distance allow.
 template <class X>
 cudaError_t launch_pack_i8(const void* x, int m, int k, int64_t ldx, void* image, float* scale, cudaStream_t st) {
-  const bool wide = ((uintptr_t)x & 15) == 0 && (m == 1 || ldx * sizeof(X) % 16 == 0);
+  const uint64_t at = (uintptr_t)x | (m == 1 ? 0 : (uint64_t)ldx * sizeof(X));
   const dim3 grid((m + 7) / 8);
-  if (wide) pack_rows_i8_kernel<X, true><<<grid, 256, 0, st>>>((const X*)x, m, k, ldx, (unsigned char*)image, scale);
-  else pack_rows_i8_kernel<X, false><<<grid, 256, 0, st>>>((const X*)x, m, k, ldx, (unsigned char*)image, scale);
+  const auto go = [&](auto kern) { kern<<<grid, 256, 0, st>>>((const X*)x, m, k, ldx, (unsigned char*)image, scale); };
+  if (at % 16 == 0) go(pack_rows_i8_kernel<X, 16>);
+  else if (at % 8 == 0) go(pack_rows_i8_kernel<X, 8>);
+  else if (at % 4 == 0) go(pack_rows_i8_kernel<X, 4>);
+  else if constexpr (sizeof(X) == 2) go(pack_rows_i8_kernel<X, 2>);
   return cudaGetLastError();
 }
 
