@@ -40,4 +40,24 @@ DEVI void store_q4_64(const float (&v)[64], uint8_t* codes, uint32_t* pair) {
   *pair = g.word;
 }
 
+// The same for 32 values already rounded to bf16, whose vector's or group's scale is known.
+DEVI void store_q8_32(const float (&f)[32], float inv, int8_t* dst) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int q = __float2int_rn(fminf(fmaxf(__fmul_rn(f[16 * c + i], inv), -127.f), 127.f));
+      w[i >> 2] |= (uint32_t)(q & 0xff) << ((i & 3) * 8);
+    }
+    *reinterpret_cast<uint4*>(dst + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+DEVI void store_q4_32(const float (&f)[32], const Kv4Group& g, uint8_t* codes) {
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) w[i >> 3] |= (uint32_t)kv4_code(kv4_clamp(f[i]), g) << ((i & 7) * 4);
+  *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 }  // namespace b200dec_detail

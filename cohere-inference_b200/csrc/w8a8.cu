@@ -6,12 +6,12 @@
 // pipeline stage is two plain cp.async.bulk copies. tcgen05.mma kind::i8 multiplies M 128 x N TN x K 32 into 32-bit integer
 // accumulators in tensor memory: the sums are exact, and every later operation rounds once.
 //   * persistent CTAs walk the (channel tile, row tile) list: warp 0 feeds the ring, warp 1 issues the MMAs into one of two
-//     accumulators, warps 2-9 drain the other: two warps per 32 lanes, each half of the tile's columns. Per k the MMA is twice as
-//     fast as with 16-bit operands, so the epilogue, not the operands, decides unless eight warps share it: a tile of 128 x 256 x
-//     1024 multiplies for about 4 100 cycles, and four warps took 24 000 to scale, round and store it.
+//     accumulators, warps 2-17 drain the other: four warps per 32 lanes, each a quarter of the tile's columns. Per k the MMA is
+//     twice as fast as with 16-bit operands, so the epilogue decides, and what decides it is latency: 13 600 x 1024 x 16 384 to bf16
+//     took 591 us with four warps, 258-274 with eight, 240 with sixteen and turned stores; the products alone take 152 us (the slope over k).
+//     Pairs of CTAs (cta_group::2), which copy a third less, were slower: 390 us per 1024 of k.
 //   * channel scales and biases of a tile go to shared memory once, as pairs, and are read back as broadcasts.
-//   * rows leave in whole 32-byte sectors, a thread per row; rows that are not 32-byte aligned through a transposition in shared
-//     memory, so that a warp's store still covers whole lines.
+//   * rows leave in runs of 64 bytes; rows that are not 16-byte aligned through a transposition in shared memory.
 // Every mbarrier wait is bounded; a wait that runs out sets B200DEC_ST_TIMEOUT, the roles fall through, copies in flight are
 // awaited (bounded) and tensor memory is released.
 #include <type_traits>
@@ -24,11 +24,13 @@ using namespace b200dec_detail;
 namespace {
 
 constexpr int BM = UMMA_BM, BN = UMMA_BN, MAX_K8 = 131072;  // 127 * 127 * k stays below 2^31
-constexpr int EPI_WARPS = 8, NTHREADS = 64 + 32 * EPI_WARPS, TR_COLS = 16, TR_LD = TR_COLS + 1;
+constexpr int EPI_WARPS = 16, NTHREADS = 64 + 32 * EPI_WARPS;
 
 template <int TN>
 struct Tile {
-  static constexpr int B_STAGE = TN * 128, STAGE_BYTES = A_STAGE + B_STAGE, STAGES = TN == 256 ? 4 : TN == 128 ? 6 : 8;
+  static constexpr int B_STAGE = TN * 128, STAGE_BYTES = A_STAGE + B_STAGE, STAGES = TN == 256 ? 4 : TN == 128 ? 5 : 7;
+  static constexpr int TR_COLS = TN == 256 ? 8 : 16, TR_LD = TR_COLS + 1;  // columns of rows turned in shared memory at a time
+  static constexpr int PARTS = TN / 32 < 4 ? TN / 32 : 4;                  // of the columns, a warp each per 32 lanes
   static constexpr int PAIRS = STAGES * STAGE_BYTES, TR = PAIRS + 2 * TN * 8;  // {scale, bias} per column and accumulator
   static constexpr int SMEM_BYTES = TR + EPI_WARPS * 32 * TR_LD * 4 + 1024;     // slack to align the base to a swizzle atom
   static constexpr int TMEM_COLS = 2 * TN;
@@ -73,17 +75,53 @@ DEVI float activate(float x, int act) {
   return x;
 }
 
-// 32 sums of a row -> values: (sum * (row scale * channel scale)) + bias, pr: the columns' {scale, bias}
-DEVI void finish32(const uint32_t (&e)[32], float* v, const float2* pr, float sa, int act) {
+// two fp32 operations in one instruction
+DEVI uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+DEVI void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+DEVI uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+DEVI uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 32 sums of a row -> values: sum * (row scale * channel scale) + bias; ws, bs: the columns' scales and biases
+DEVI void finish32(const uint32_t (&e)[32], float (&v)[32], const float* ws, const float* bs, float sa, int act) {
+  const uint64_t s2 = pack2(sa, sa);
 #pragma unroll
-  for (int i = 0; i < 32; i += 2) {
-    const float4 p = *reinterpret_cast<const float4*>(pr + i);
-    v[i] = __fadd_rn(__fmul_rn(__int2float_rn((int)e[i]), __fmul_rn(sa, p.x)), p.y);
-    v[i + 1] = __fadd_rn(__fmul_rn(__int2float_rn((int)e[i + 1]), __fmul_rn(sa, p.z)), p.w);
+  for (int i = 0; i < 32; i += 4) {
+    const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(ws + i), b = *reinterpret_cast<const ulonglong2*>(bs + i);
+    unpack2(fma2(pack2(__int2float_rn((int)e[i]), __int2float_rn((int)e[i + 1])), mul2(s2, w.x), b.x), v[i], v[i + 1]);
+    unpack2(fma2(pack2(__int2float_rn((int)e[i + 2]), __int2float_rn((int)e[i + 3])), mul2(s2, w.y), b.y), v[i + 2], v[i + 3]);
   }
   if (act != B200DEC_ACT_NONE) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = activate(v[i], act);
+  }
+}
+
+// Among four neighbouring lanes, each with four pieces of 16 bytes: piece j of lane i becomes piece i of lane j.
+DEVI void turn_pieces(uint32_t (&p)[4][4], int lane) {
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    const bool high = lane & o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j & o) continue;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? p[j][c] : p[j + o][c], o);
+        p[j][c] = high ? got : p[j][c], p[j + o][c] = high ? p[j + o][c] : got;
+      }
+    }
   }
 }
 
@@ -98,51 +136,47 @@ DEVI uint32_t pair_of(float a, float b, __half) {
   return reinterpret_cast<const uint32_t&>(h);
 }
 DEVI uint32_t pair_of(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
-DEVI void st_sector(void* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
-               "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
-}
-
 // 32 columns of the warp's 32 rows (a row per thread) from row m0 on, column n0 on, into T rows
-template <class T>
-DEVI void store_rows(const W8Args& p, const float* v, int m0, int n0, int lane, bool wide, float* tr) {
+template <class T, int TR_COLS>
+DEVI void store_rows(const W8Args& p, const float (&v)[32], int m0, int n0, int lane, bool wide, float* tr) {
+  constexpr int TR_LD = TR_COLS + 1, ROWS = 32 / TR_COLS;
   T* out = reinterpret_cast<T*>(p.out);
   if (wide && n0 + 32 <= p.N) {
-    if (m0 + lane < p.M) {
-      T* d = out + (size_t)(m0 + lane) * p.ldo + n0;
-      if constexpr (sizeof(T) == 4) {
+    // 64 bytes of a row at a time: four lanes turn theirs, so that a store instruction covers runs of 64 bytes of eight rows (a
+    // thread per row wrote 32 rows' single sectors: 267 us for 13 600 x 1024 x 16 384, 240 this way)
+    constexpr int PER = 16 / (int)sizeof(T);  // values of a piece
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[8];
+    for (int c = 0; c < 32; c += 4 * PER) {
+      uint32_t w[4][4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * c + i]);
-          st_sector(d + 8 * c, w);
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (sizeof(T) == 4) w[j][i] = __float_as_uint(v[c + PER * j + i]);
+          else w[j][i] = pair_of(v[c + PER * j + 2 * i], v[c + PER * j + 2 * i + 1], T());
         }
-      } else {
+      turn_pieces(w, lane);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = pair_of(v[16 * c + 2 * i], v[16 * c + 2 * i + 1], T());
-          st_sector(d + 16 * c, w);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const int m = m0 + (lane & ~3) + j;
+        if (m < p.M)
+          *reinterpret_cast<uint4*>(out + (size_t)m * p.ldo + n0 + c + PER * (lane & 3)) = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
       }
     }
     return;
   }
-  // 16 columns at a time through shared memory: a store instruction then covers two rows' runs of 16 columns
+  // TR_COLS columns at a time through shared memory: a store instruction then covers runs of that many columns
 #pragma unroll
   for (int c = 0; c < 32; c += TR_COLS) {
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < TR_COLS; ++i) tr[lane * TR_LD + i] = v[c + i];
     __syncwarp();
-    const int col = n0 + c + (lane & 15);
+    const int col = n0 + c + lane % TR_COLS;
     if (col < p.N) {
 #pragma unroll 4
-      for (int r = lane >> 4; r < 32; r += 2)
-        if (m0 + r < p.M) out[(size_t)(m0 + r) * p.ldo + col] = out_value<T>(tr[r * TR_LD + (lane & 15)]);
+      for (int r = lane / TR_COLS; r < 32; r += ROWS)
+        if (m0 + r < p.M) out[(size_t)(m0 + r) * p.ldo + col] = out_value<T>(tr[r * TR_LD + lane % TR_COLS]);
     }
   }
 }
@@ -243,12 +277,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) w8a8_kernel(const W8Args p) {
       if (!ok) atomicOr(p.status, B200DEC_ST_TIMEOUT);
     }
   } else {
-    // ---- epilogue: warp w reads tensor-memory lanes 32 (w % 4) .. + 31, the first four the low half of the columns ----------
-    const int q = warp & 3, row = q * 32 + lane, half = (warp - 2) >> 2, et = tid - 64;
-    constexpr int HALF = TN / 2;
-    float* tr = reinterpret_cast<float*>(smem + Cfg::TR) + (warp - 2) * 32 * TR_LD;
+    // ---- epilogue: warp w reads tensor-memory lanes 32 (w % 4) .. + 31, the columns' part (w - 2) / 4 -----------------------
+    const int q = warp & 3, row = q * 32 + lane, part = (warp - 2) >> 2, et = tid - 64;
+    // rows: every part a warp of its own; caches: two parts, so that a head's 128 channels are one thread's
+    const int parts = p.mode == 4 ? Cfg::PARTS : 2, cols = TN / parts;
+    float* tr = reinterpret_cast<float*>(smem + Cfg::TR) + (warp - 2) * 32 * Cfg::TR_LD;
     const int size = p.out_kind == B200DEC_T_F32 ? 4 : 2;
-    const bool wide = ((uintptr_t)p.out & 31) == 0 && p.ldo * size % 32 == 0;
+    const bool wide = ((uintptr_t)p.out & 15) == 0 && p.ldo * size % 16 == 0;
     bool ok = true;
     uint32_t tc = 0;
     // what a tile needs from global memory is fetched a tile ahead: this thread's column's {scale, bias}, its row's scale
@@ -266,8 +301,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) w8a8_kernel(const W8Args p) {
       const int mt = (int)(tile % MT), nt = (int)(tile / MT), buf = tc & 1;
       const int m = mt * BM + row;
       // the pairs go into the buffer of two tiles ago, which every warp has left (it passed the barrier of the tile between)
-      float2* pairs = reinterpret_cast<float2*>(smem + Cfg::PAIRS) + buf * TN;
-      if (et < TN) pairs[et] = pair_next;
+      float* pairs = reinterpret_cast<float*>(smem + Cfg::PAIRS) + buf * 2 * TN;  // TN scales, TN biases
+      if (et < TN) pairs[et] = pair_next.x, pairs[TN + et] = pair_next.y;
       const float sa = sa_next;
       fetch(tile + gridDim.x);
       int slot = -1, frame = 0;
@@ -286,76 +321,71 @@ __global__ void __launch_bounds__(NTHREADS, 1) w8a8_kernel(const W8Args p) {
       if (ok) ok = mbar_wait(&tfull[buf], (tc >> 1) & 1);
       if (!ok) continue;
       tc_fence_after();
-      const uint32_t acc = tmem_d + buf * TN + half * HALF + ((uint32_t)(q * 32) << 16);
-      const float2* pr = pairs + half * HALF;
-      const int n0 = nt * TN + half * HALF;
+      const uint32_t acc = tmem_d + buf * TN + part * cols + ((uint32_t)(q * 32) << 16);
+      const float* ws = pairs + part * cols;
+      const float* bs = ws + TN;
+      const int n0 = nt * TN + part * cols;
+      const auto load = [&](int c, float (&v)[32], int act) {  // columns c .. c + 31 of the part
+        uint32_t e[32];
+        __syncwarp();  // a collective load: rows without a slot may have gone ahead
+        tmem_ld32(acc + c, e);
+        tmem_wait();
+        finish32(e, v, ws + c, bs + c, sa, act);
+      };
+      float v[32];
       if (p.mode == 4) {
-        uint32_t e[2][32];
-        tmem_ld32(acc, e[0]);
-#pragma unroll
-        for (int c = 0; c < HALF / 32; ++c) {
-          tmem_wait();
-          if (c + 1 < HALF / 32) tmem_ld32(acc + 32 * (c + 1), e[(c + 1) & 1]);
-          if (n0 + 32 * c >= p.N) continue;
-          float v[32];
-          finish32(e[c & 1], v, pr + 32 * c, sa, p.act);
-          if (p.out_kind == B200DEC_T_F32) store_rows<float>(p, v, mt * BM + q * 32, n0 + 32 * c, lane, wide, tr);
-          else if (p.out_kind == B200DEC_T_F16) store_rows<__half>(p, v, mt * BM + q * 32, n0 + 32 * c, lane, wide, tr);
-          else store_rows<__nv_bfloat16>(p, v, mt * BM + q * 32, n0 + 32 * c, lane, wide, tr);
-        }
-      } else if constexpr (TN == BN) {
-        // caches: 64 channels at a time; channel n = ((layer * 2 + k|v) * H + head) * D + d
-        const auto load64 = [&](int c, float (&v)[64]) {
-          uint32_t e[2][32];
-          tmem_ld32(acc + c, e[0]);
-          tmem_ld32(acc + c + 32, e[1]);
-          tmem_wait();
-          finish32(e[0], v, pr + c, sa, B200DEC_ACT_NONE);
-          finish32(e[1], v + 32, pr + c + 32, sa, B200DEC_ACT_NONE);
-        };
+        if (part < parts)
 #pragma unroll 1
-        for (int c = 0; c < HALF; c += 64) {
+          for (int c = 0; c < TN / Cfg::PARTS && n0 + c < p.N; c += 32) {
+            load(c, v, p.act);
+            const int m0 = mt * BM + q * 32;
+            if (p.out_kind == B200DEC_T_F32) store_rows<float, Cfg::TR_COLS>(p, v, m0, n0 + c, lane, wide, tr);
+            else if (p.out_kind == B200DEC_T_F16) store_rows<__half, Cfg::TR_COLS>(p, v, m0, n0 + c, lane, wide, tr);
+            else store_rows<__nv_bfloat16, Cfg::TR_COLS>(p, v, m0, n0 + c, lane, wide, tr);
+          }
+      } else if constexpr (TN == BN) {
+        // caches: a group of 64 channels, or a head's D for int8, at a time; channel n = ((layer * 2 + k|v) * H + head) * D + d.
+        // Its values go by twice, for its extremes and to be stored.
+        const int span = p.mode == 2 ? p.D : 64;
+#pragma unroll 1
+        for (int c = 0; c < cols && part < parts; c += span) {
           const int n = n0 + c, hd = p.H * p.D, l = n / (2 * hd), kvi = (n / hd) & 1, h = (n % hd) / p.D, d0 = n % p.D;
           const size_t vec = slot < 0 ? 0 : ((((size_t)l * p.S1 + slot) * p.H + h) * p.T + frame);
-          float v[64];
-          load64(c, v);
-          if (p.mode == 1) {
-            if (slot >= 0) {
-              __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(kvi ? p.cv : p.ck) + vec * p.D + d0;
+          char* cache = reinterpret_cast<char*>(kvi ? p.cv : p.ck);
+          float mn = INFINITY, mx = -INFINITY;
+          if (p.mode != 1) {
+#pragma unroll 1
+            for (int i = 0; i < span; i += 32) {
+              load(c + i, v, B200DEC_ACT_NONE);
 #pragma unroll
-              for (int i = 0; i < 64; i += 8)
-                *reinterpret_cast<uint4*>(dst + i) = make_uint4(pack_bf16(v[i], v[i + 1]), pack_bf16(v[i + 2], v[i + 3]),
-                                                                pack_bf16(v[i + 4], v[i + 5]), pack_bf16(v[i + 6], v[i + 7]));
-            }
-          } else if (p.mode == 3) {
-            if (slot >= 0)
-              store_q4_64(v, reinterpret_cast<uint8_t*>(kvi ? p.cv : p.ck) + (vec * p.D + d0) / 2,
-                          reinterpret_cast<uint32_t*>(kvi ? p.cvs : p.cks) + (vec * p.D + d0) / 64);
-          } else {
-            // int8: the vector's largest magnitude over its 64 or 128 channels (a half of the columns holds a whole vector)
-            float mx = 0.f;
-#pragma unroll
-            for (int i = 0; i < 64; ++i) {
-              v[i] = __bfloat162float(__float2bfloat16_rn(v[i]));
-              mx = fmaxf(mx, fabsf(v[i]));
-            }
-            int8_t* dst = reinterpret_cast<int8_t*>(kvi ? p.cv : p.ck) + vec * p.D + d0;
-            if (p.D == 128) {
-              float u[64];
-              load64(c + 64, u);
-#pragma unroll
-              for (int i = 0; i < 64; ++i) {
-                u[i] = __bfloat162float(__float2bfloat16_rn(u[i]));
-                mx = fmaxf(mx, fabsf(u[i]));
+              for (int j = 0; j < 32; ++j) {
+                const float b = __bfloat162float(__float2bfloat16_rn(v[j])), x = p.mode == 3 ? kv4_clamp(b) : b;
+                mn = fminf(mn, x), mx = fmaxf(mx, x);
               }
-              if (slot >= 0) store_q8_64(u, mx, dst + 64);
-              c += 64;
-            }
-            if (slot >= 0) {
-              store_q8_64(v, mx, dst);
-              (kvi ? p.cvs : p.cks)[vec] = mx > 0.f ? __fdiv_rn(mx, 127.f) : 1.f;
             }
           }
+          const float top = fmaxf(fmaxf(mx, -mn), 0.f), s8 = top > 0.f ? __fdiv_rn(top, 127.f) : 1.f, inv8 = __fdiv_rn(1.f, s8);
+          const Kv4Group g = kv4_group(mn, mx);
+#pragma unroll 1
+          for (int i = 0; i < span; i += 32) {
+            load(c + i, v, B200DEC_ACT_NONE);
+            if (slot >= 0) {
+              const size_t at = vec * p.D + d0 + i;
+              if (p.mode == 1) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 8)
+                  *reinterpret_cast<uint4*>(cache + (at + j) * 2) = make_uint4(pack_bf16(v[j], v[j + 1]), pack_bf16(v[j + 2], v[j + 3]),
+                                                                               pack_bf16(v[j + 4], v[j + 5]), pack_bf16(v[j + 6], v[j + 7]));
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
+                if (p.mode == 2) store_q8_32(v, inv8, reinterpret_cast<int8_t*>(cache) + at);
+                else store_q4_32(v, g, reinterpret_cast<uint8_t*>(cache) + at / 2);
+              }
+            }
+          }
+          if (slot >= 0 && p.mode == 2) (kvi ? p.cvs : p.cks)[vec] = s8;
+          if (slot >= 0 && p.mode == 3) reinterpret_cast<uint32_t*>(kvi ? p.cvs : p.cks)[(vec * p.D + d0) / 64] = g.word;
         }
       }
       tc_fence_before();
