@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(NTHREADS) attention_q4_kernel(const Q4Args p) 
     for (int i = 0; i < D / 32; ++i) {
       if (i % WPI != wi) continue;
       const int d = 32 * i + lane, at = (d & ~7) + 2 * (d & 3) + ((d >> 2) & 1);  // dims d and d + 4 of a word side by side
-      const float v = rintf(x[i] * (f * p.scale_log2));                           // |v| <= 2^22
+      const float v = rintf(x[i] * p.scale_log2 * f);                             // |v| <= 2^22
       const float hi = rintf(v * 0.00048828125f), lo = v - 2048.f * hi;           // |hi| <= 2^11, |lo| <= 2^10
       const float sc = (d & 1) ? 0.0625f : 1.f;
       s_q[it][0][at] = __float2half_rn(hi * sc), s_q[it][1][at] = __float2half_rn(lo * sc);
@@ -506,6 +506,7 @@ int b200dec_attention_q4(int self, const int32_t* active, const float* q, int ld
   B200_REQUIRE(head_dim == 64 || head_dim == 128, "attention_q4: head_dim %d (64 or 128)", head_dim);
   B200_REQUIRE(rows >= 1 && rows <= 65535 && heads >= 1 && heads <= 65535 && cap >= 1 && cap <= 1 << 30 && slots >= 0,
                "attention_q4: rows %d heads %d cap %d slots %d", rows, heads, cap, slots);
+  B200_REQUIRE((int64_t)rows * heads <= 1 << 26, "attention_q4: %d rows x %d heads", rows, heads);
   B200_REQUIRE(ldq >= (self ? 3 : 1) * heads * head_dim && ldq % 4 == 0 && ((uintptr_t)q & 15) == 0,
                "attention_q4: ldq %d (rows of %d floats, 16-byte aligned)", ldq, (self ? 3 : 1) * heads * head_dim);
   B200_REQUIRE((((uintptr_t)kcache | (uintptr_t)vcache) & 15) == 0 && ((uintptr_t)kpairs | (uintptr_t)vpairs) % (head_dim / 16) == 0 &&

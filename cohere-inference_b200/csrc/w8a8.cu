@@ -24,6 +24,7 @@ using namespace b200dec_detail;
 namespace {
 
 constexpr int BM = UMMA_BM, BN = UMMA_BN, MAX_K8 = 131072;  // 127 * 127 * k stays below 2^31
+constexpr int MAX_MN = 1 << 30;
 constexpr int EPI_WARPS = 16, NTHREADS = 64 + 32 * EPI_WARPS;
 
 template <int TN>
@@ -581,18 +582,18 @@ int launch(const W8Args& a, cudaStream_t stream) {
 extern "C" {
 
 int64_t b200dec_w8a8_rows_bytes(int m, int k) {
-  if (m < 0 || k <= 0 || k > MAX_K8) return -1;
+  if (m < 0 || m > MAX_MN || k <= 0 || k > MAX_K8) return -1;
   return (int64_t)((m + BM - 1) / BM) * BM * ((k + 127) / 128 * 128);
 }
 
 int64_t b200dec_w8a8_weight_bytes(int n, int k) {
-  if (n <= 0 || k <= 0 || k > MAX_K8) return -1;
+  if (n <= 0 || n > MAX_MN || k <= 0 || k > MAX_K8) return -1;
   return (int64_t)((n + BN - 1) / BN) * BN * ((k + 127) / 128 * 128);
 }
 
 int b200dec_w8a8_pack_rows(const void* x, int kind, int m, int k, int64_t ldx, void* image, float* scale, void* stream) {
   B200_REQUIRE(x && image && scale, "w8a8_pack_rows: null pointer");
-  B200_REQUIRE(m >= 1 && k >= 1 && k <= MAX_K8 && (m == 1 || ldx >= k), "w8a8_pack_rows: m %d k %d ldx %lld", m, k, (long long)ldx);
+  B200_REQUIRE(m >= 1 && m <= MAX_MN && k >= 1 && k <= MAX_K8 && (m == 1 || ldx >= k), "w8a8_pack_rows: m %d k %d ldx %lld", m, k, (long long)ldx);
   B200_REQUIRE(kind == B200DEC_T_F32 || kind == B200DEC_T_F16 || kind == B200DEC_T_BF16, "w8a8_pack_rows: kind %d", kind);
   B200_REQUIRE(((uintptr_t)image & 1023) == 0 && (uintptr_t)x % (kind == B200DEC_T_F32 ? 4 : 2) == 0,
                "w8a8_pack_rows: alignment (the image 1 KB)");
@@ -605,7 +606,7 @@ int b200dec_w8a8_pack_rows(const void* x, int kind, int m, int k, int64_t ldx, v
 }
 
 int b200dec_w8a8_tile_weight(const int8_t* q, int n, int k, void* image, void* stream) {
-  B200_REQUIRE(q && image && n >= 1 && k >= 1 && k <= MAX_K8 && ((uintptr_t)image & 1023) == 0,
+  B200_REQUIRE(q && image && n >= 1 && n <= MAX_MN && k >= 1 && k <= MAX_K8 && ((uintptr_t)image & 1023) == 0,
                "w8a8_tile_weight: (%d, %d) into a 1 KB aligned image", n, k);
   const size_t total = (size_t)b200dec_w8a8_weight_bytes(n, k) / 16;
   tile_weight_i8_kernel<<<(unsigned)((total + 255) / 256), 256, 0, (cudaStream_t)stream>>>(q, n, k, (unsigned char*)image);
@@ -616,7 +617,7 @@ int b200dec_w8a8_linear(const void* rows_image, const float* row_scale, int m, i
                         const float* w_scale, const float* bias, int n, int act, void* out, int out_kind, int64_t ldo,
                         int32_t* status, void* stream) {
   B200_REQUIRE(rows_image && row_scale && weight_image && w_scale && out && status, "w8a8_linear: null pointer");
-  B200_REQUIRE(m >= 1 && n >= 1 && k >= 1 && k <= MAX_K8 && (m == 1 || ldo >= n), "w8a8_linear: m %d k %d n %d ldo %lld", m, k, n,
+  B200_REQUIRE(m >= 1 && m <= MAX_MN && n >= 1 && n <= MAX_MN && k >= 1 && k <= MAX_K8 && (m == 1 || ldo >= n), "w8a8_linear: m %d k %d n %d ldo %lld", m, k, n,
                (long long)ldo);
   B200_REQUIRE(out_kind == B200DEC_T_F32 || out_kind == B200DEC_T_F16 || out_kind == B200DEC_T_BF16, "w8a8_linear: out_kind %d", out_kind);
   B200_REQUIRE(act == B200DEC_ACT_NONE || act == B200DEC_ACT_RELU || act == B200DEC_ACT_GELU, "w8a8_linear: act %d", act);
@@ -635,7 +636,7 @@ int b200dec_w8a8_prefill(const void* rows_image, const float* row_scale, int m, 
                          void* cv, void* ck_scale, void* cv_scale, int layers, int slots_plus_1, int heads, int head_dim, int frames,
                          int32_t* status, void* stream) {
   B200_REQUIRE(rows_image && row_scale && weight_image && w_scale && status, "w8a8_prefill: null pointer");
-  B200_REQUIRE(m >= 1 && k >= 1 && k <= MAX_K8 && mode >= 1 && mode <= 3, "w8a8_prefill: m %d k %d mode %d", m, k, mode);
+  B200_REQUIRE(m >= 1 && m <= MAX_MN && k >= 1 && k <= MAX_K8 && mode >= 1 && mode <= 3, "w8a8_prefill: m %d k %d mode %d", m, k, mode);
   B200_REQUIRE(pieces && n_pieces >= 1 && ck && cv && (mode == 1 || (ck_scale && cv_scale)), "w8a8_prefill: pieces and caches");
   B200_REQUIRE((((uintptr_t)rows_image | (uintptr_t)weight_image) & 1023) == 0 &&
                    (((uintptr_t)w_scale | (uintptr_t)bias | (uintptr_t)pieces | (uintptr_t)ck | (uintptr_t)cv) & 15) == 0,

@@ -388,6 +388,8 @@ class StreamDecoder:
         po = man["pack_options"]
         if "umma_above_rows" in kw:
             raise ValueError("umma_above_rows is a packing option: it comes from the file")
+        if "prefill_int8" in kw:
+            raise ValueError("prefill_int8 is a packing option: it comes from the file")
         self = cls(shim, int8=po["int8"], fp16_weights=po.get("fp16_weights", False), ffn_sparse=po["ffn_sparse"],
                    head_split=po["head_split"], umma_above_rows=po.get("small_rows", 0),
                    head_umma=po["head_umma"], proj_umma=po["proj_umma"] or False,

@@ -372,7 +372,8 @@ int b200dec_scatter_kv_q8(const float* kv, const int32_t* slot_of, const int32_t
 /* b200dec_attention over 4-bit caches, for any cap: heads x head_dim as the caches have them, n[s] = 0 .. cap - 1 cached keys
  * (self != 0: the row's new key and value are written at n[s] and attended in this step as bf16 values) or 0 .. cap frames
  * (a row without any gives zeros). Scores, softmax and sums in fp32. sched: NULL, or a table of b200dec_row_schedule
- * (16-byte aligned; active, n and status are then not read). part, count: a workspace of
+ * (16-byte aligned; active, n and status are then not read). Alignment: q and the codes 16 bytes, pairs D / 16, ldq a multiple of
+ * 4. part, count: a workspace of
  * b200dec_attention_q4_scratch_floats() floats and rows * heads counters, zero on entry and on exit, for the calls of one
  * stream at a time (two captured graphs that may run side by side need one each); both NULL: a row is one CTA however
  * long it is. Two rows of one call must not append to the same slot, the dummy excepted. */
@@ -408,7 +409,8 @@ int b200dec_logit_rules(const void* logits, int kind, int64_t ldl, int rows, int
  * out (m, n) = act((q w^T) * row scale * channel scale + bias): rows quantised as they come, one scale each (s = max(max |x|,
  * 1e-12) / 127, q = rint(x / s), NaN for a row that holds an infinity or NaN), int8 weights with one scale per channel
  * (b200dec_quantize_rows), exact 32-bit sums, every later operation rounded once in fp32. Any m, n; k <= 131072. The operands
- * are images of their shared-memory tiles, 1 KB aligned. The reference multiplies int8 weights with 16-bit rows
+ * are images of their shared-memory tiles, 1 KB aligned. The products start on their weights while the kernel before them on the
+ * stream still runs: an image and its scales are init-time data, complete before that kernel starts. The reference multiplies int8 weights with 16-bit rows
  * (kernels/csrc/dec_w8.cu:46-234), as b200dec_linear does; this is the form for many rows. */
 int64_t b200dec_w8a8_rows_bytes(int m, int k);
 int64_t b200dec_w8a8_weight_bytes(int n, int k);
@@ -416,7 +418,7 @@ int64_t b200dec_w8a8_weight_bytes(int n, int k);
 int b200dec_w8a8_pack_rows(const void* x, int kind, int m, int k, int64_t ldx, void* image, float* scale, void* stream);
 /* q (n, k) int8 row-major -> image; init time. */
 int b200dec_w8a8_tile_weight(const int8_t* q, int n, int k, void* image, void* stream);
-/* w_scale (n) and bias (n) or NULL 16-byte aligned, act B200DEC_ACT_*, out (m, ldo) of out_kind (B200DEC_T_*). status receives
+/* m, n <= 2^30; w_scale (n) and bias (n) or NULL 16-byte aligned, act B200DEC_ACT_*, out (m, ldo) of out_kind (B200DEC_T_*). status receives
  * B200DEC_ST_TIMEOUT if a bounded wait inside the kernel ran out. */
 int b200dec_w8a8_linear(const void* rows_image, const float* row_scale, int m, int k, const void* weight_image,
                         const float* w_scale, const float* bias, int n, int act, void* out, int out_kind, int64_t ldo,

@@ -31,6 +31,7 @@ ATTEND = dict(self=1, active=A, q=A, ldq=3 * 1024, k=A, v=A, km=A, vm=A, n=A, sc
     (dict(cap=(1 << 30) + 1), "cap"), (dict(slots=-1), "slots"), (dict(ldq=3 * 1024 - 4), "ldq"), (dict(ldq=3 * 1024 + 2), "ldq"),
     (dict(self=0, ldq=1020), "ldq"), (dict(q=A + 4), "ldq"), (dict(k=A + 8), "alignment"), (dict(km=A + 2), "alignment"),
     (dict(sched=A + 4), "alignment"), (dict(kind=2), "out_kind"),
+    (dict(rows=65535, heads=8192, ldq=3 * 8192 * 128), "rows x"), (dict(dim=128, km=A + 4), "alignment"),
 ])
 def test_attention_q4(nv, change, text):
     refused(nv, nv.lib().b200dec_attention_q4(*{**ATTEND, **change}.values()), text)
@@ -100,7 +101,7 @@ LINEAR = dict(rows_image=A, row_scale=A, m=4, k=64, weight=A, w_scale=A, bias=No
 @pytest.mark.parametrize("change, text", [
     (dict(rows_image=None), "null"), (dict(row_scale=None), "null"), (dict(weight=None), "null"), (dict(w_scale=None), "null"),
     (dict(out=None), "null"), (dict(status=None), "null"), (dict(m=0), "m 0"), (dict(n=0), "n 0"), (dict(k=0), "k 0"),
-    (dict(k=131073), "k 131073"), (dict(ldo=9), "ldo"), (dict(kind=3), "out_kind"), (dict(act=3), "act"),
+    (dict(k=131073), "k 131073"), (dict(ldo=9), "ldo"), (dict(m=(1 << 30) + 1), "m "), (dict(n=(1 << 30) + 1, ldo=1 << 31), "n "), (dict(kind=3), "out_kind"), (dict(act=3), "act"),
     (dict(rows_image=A + 512), "alignment"), (dict(weight=A + 16), "alignment"), (dict(w_scale=A + 4), "alignment"),
     (dict(bias=A + 8), "alignment"), (dict(out=A + 2), "alignment"),
 ])
