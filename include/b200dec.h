@@ -382,7 +382,7 @@ int b200dec_attention_q4(int self, const int32_t* active, const float* q, int ld
                          float scale, void* out, int out_kind, int rows, float* part, int32_t* count, int32_t* status, int pdl,
                          void* stream);
 int64_t b200dec_attention_q4_scratch_floats(int rows, int heads, int head_dim, int cap);
-/* b200dec_scatter_kv into 4-bit caches: kv (nrows, L * 2 * H * D) fp32, 32-byte aligned; codes (L, slots + 1, H, frames,
+/* b200dec_scatter_kv into 4-bit caches: kv (nrows, L * 2 * H * D) fp32, 32-byte aligned (codes 8, pairs 4); codes (L, slots + 1, H, frames,
  * D / 2), pairs (L, slots + 1, H, frames, D / 64, 2). Rows whose slot or frame is outside the caches are dropped; no two rows
  * may have the same slot and frame. */
 int b200dec_scatter_kv_q4(const float* kv, const int32_t* slot_of, const int32_t* frame_of, void* ck, void* cv, void* ck_pairs,
