@@ -1,8 +1,8 @@
 // Rows of keys and values into the 4-bit slot caches, and back (format: kv4.cuh).
 //
 // One thread per 16 dims on the way in (two 32-byte loads, the group's extremes over four lanes; what a group costs is shared by
-// more values than with 8), per 8 on the way back; the first lane of a group stores its (step, lo). A CTA takes a fixed range of channels over many rows, so that the channel's (layer, key | value, head) is
-// worked out once. What it has to move is the fp32 rows (8 times the codes); the way in is close to bound by its instructions (23
+// more values than with 8), per 8 on the way back; the first lane of a group stores its (step, lo). A CTA takes a fixed range
+// of channels over many rows, so that the channel's (layer, key | value, head) is worked out once. What it has to move is the fp32 rows (8 times the codes); the way in is close to bound by its instructions (23
 // a value), the way back by writing. 64 clips, 13 600 rows of 16 384 values: 179 us in (5.7 TB/s; 217 with 8 dims a
 // thread), 171 us back (5.9 TB/s).
 #include "kv4.cuh"
@@ -59,17 +59,7 @@ DEVI Channel channel(const Kv4Args& p) {
 DEVI int64_t vecs(const Channel& c, int slot, int frame) { return (int64_t)slot * c.slot_vecs + frame; }
 DEVI bool inside(const Kv4Args& p, int slot, int frame) { return slot >= 0 && slot < p.S1 && frame >= 0 && frame < p.T; }
 
-// The extremes of a thread's 8 values go round in bf16, the largest and the negated smallest in one word.
-DEVI uint32_t max_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 m = __hmax2_nan(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
-  return reinterpret_cast<const uint32_t&>(m);
-}
-DEVI uint32_t min_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 m = __hmin2_nan(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
-  return reinterpret_cast<const uint32_t&>(m);
-}
-
-__global__ void __launch_bounds__(THREADS) scatter_kv_q4_kernel(const Kv4Args p) {
+__global__ void __launch_bounds__(THREADS, 4) scatter_kv_q4_kernel(const Kv4Args p) {
   const Channel c = channel<16>(p);
   const size_t width = (size_t)p.L * 2 * p.H * p.D, at = (size_t)(blockIdx.x * THREADS + threadIdx.x) * 16;
   struct Row {
@@ -99,13 +89,12 @@ __global__ void __launch_bounds__(THREADS) scatter_kv_q4_kernel(const Kv4Args p)
         hi = k + i ? max_bf16x2(hi, w) : w, lo = k + i ? min_bf16x2(lo, w) : w;
         r.x[k].v[i] = bf16_lo(w), r.x[k].v[i + 1] = bf16_hi(w);
       }
-    // {largest, -smallest} of the 16, then of the group's four threads
+    // {largest, -smallest} of the 16, then of the group's four threads: both go round in one word
     uint32_t ext = max_bf16x2(__byte_perm(hi, lo ^ 0x80008000u, 0x5410), __byte_perm(hi, lo ^ 0x80008000u, 0x7632));
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) ext = max_bf16x2(ext, __shfl_xor_sync(0xffffffffu, ext, o));
     float mx = bf16_lo(ext), mn = -bf16_hi(ext);
-    const bool tame = mx <= KV4_LIMIT && mn >= -KV4_LIMIT;  // false for a NaN too
-    if (__any_sync(0xffffffffu, !tame)) {  // something to clamp, or a NaN, in some group of the warp
+    if (__any_sync(0xffffffffu, !kv4_tame(mn, mx))) {  // something to clamp, or a NaN, in some group of the warp
       mn = INFINITY, mx = -INFINITY;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -126,17 +115,8 @@ __global__ void __launch_bounds__(THREADS) scatter_kv_q4_kernel(const Kv4Args p)
     const bool plain = kv4_plain(g);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      if (plain) codes[k] = kv4_codes8(r.x[k].v, g);
-      else {
-        codes[k] = 0;
-#pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-          float x = r.x[k].v[0];  // the first, the rest move up: no index into registers
-#pragma unroll
-          for (int j = 0; j < 7; ++j) r.x[k].v[j] = r.x[k].v[j + 1];
-          codes[k] |= (uint32_t)kv4_code(x, g) << (4 * i);
-        }
-      }
+      if (plain) codes[k] = kv4_codes8<false>(r.x[k].v, g);
+      else kv4_codes_slow<8, false>(r.x[k].v, g, &codes[k]);
     }
     const int64_t v = vecs(c, r.slot, r.frame);
     *reinterpret_cast<uint2*>(c.codes + v * c.code_words) = make_uint2(codes[0], codes[1]);

@@ -43,11 +43,47 @@ DEVI int kv4_code(float x, const Kv4Group& g) {
   if (-e2 > g.step || (-e2 == g.step && odd)) c -= 1.f;
   return g.step > 0.f ? (int)fminf(fmaxf(c, 0.f), 15.f) : 0;
 }
+// Largest and smallest of bf16 pairs; a NaN stays one.
+DEVI uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2_nan(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
+  return reinterpret_cast<const uint32_t&>(m);
+}
+DEVI uint32_t min_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmin2_nan(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
+  return reinterpret_cast<const uint32_t&>(m);
+}
+// Nothing to clamp, and no NaN among what the extremes are of.
+DEVI bool kv4_tame(float mn, float mx) { return mx <= KV4_LIMIT && mn >= -KV4_LIMIT; }
+
+// N values' codes the long way, in little code: the first is taken, the rest move up (no index into registers).
+template <int N, bool CLAMP>
+DEVI void kv4_codes_slow(const float* v, const Kv4Group& g, uint32_t* words) {
+  float x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = v[i];
+  uint32_t w[N / 8];
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) w[i] = 0;
+#pragma unroll 1
+  for (int i = 0; i < N; ++i) {
+    const uint32_t code = kv4_code(CLAMP ? kv4_clamp(x[0]) : x[0], g);
+#pragma unroll
+    for (int j = 0; j + 1 < N; ++j) x[j] = x[j + 1];
+    // the words move on by four bits, a new code coming in at the top: after N of them each is in its place
+#pragma unroll
+    for (int j = 0; j < N / 8; ++j) w[j] = __funnelshift_r(w[j], j + 1 < N / 8 ? w[j + 1] : code, 4);
+  }
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) words[i] = w[i];
+}
+
 // The group's pair and 8 of its values' codes, of values that are finite and within the limit, where |lo| <= 512 steps and the step
 // is a normal fp16 number (else false: the caller takes kv4_code for each). Then 0 <= x - lo + step / 2 and (x - lo) / step <=
 // 15.01, so nothing has to be clamped, and only a quotient within 2^-17 of a half needs the exact remainder. Adding 1.5 * 2^23
 // rounds to an integer, which the sum's low bits are.
 DEVI bool kv4_plain(const Kv4Group& g) { return g.step >= 6.103515625e-05f && fabsf(g.lo) <= 512.f * g.step; }
+// COMPACT: that in a loop instead of straight-line code (a kernel of few warps waits for its instructions; one of many does not).
+template <bool COMPACT>
 DEVI uint32_t kv4_codes8(const float (&x)[8], const Kv4Group& g) {
   constexpr float MAGIC = 12582912.f;  // 0x4b400000
   uint32_t w = 0;
@@ -60,9 +96,13 @@ DEVI uint32_t kv4_codes8(const float (&x)[8], const Kv4Group& g) {
   }
   w -= 0x4b400000u * 0x11111111u;
   if (near > 0.5f - 7.62939453e-06f) {
-    w = 0;
+    if constexpr (COMPACT) {
+      kv4_codes_slow<8, false>(x, g, &w);
+    } else {
+      w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= (uint32_t)kv4_code(x[i], g) << (4 * i);
+      for (int i = 0; i < 8; ++i) w |= (uint32_t)kv4_code(x[i], g) << (4 * i);
+    }
   }
   return w;
 }

@@ -20,27 +20,50 @@ DEVI void store_q8_64(const float (&f)[64], float mx, int8_t* dst) {
   }
 }
 
-// 64 values, which are one group of the 4-bit format: its codes and its pair
-DEVI void store_q4_64(const float (&v)[64], uint8_t* codes, uint32_t* pair) {
-  float mn = INFINITY, mx = -INFINITY;
+// 4 bits. The extremes of 32 values after rounding to bf16, on top of those in hi and lo (pairs; `first`: there are none yet).
+DEVI void extremes_32(const float* v, bool first, uint32_t& hi, uint32_t& lo) {
 #pragma unroll
-  for (int i = 0; i < 64; ++i) {
+  for (int i = 0; i < 32; i += 2) {
+    const uint32_t w = pack_bf16(v[i], v[i + 1]);
+    hi = first && i == 0 ? w : max_bf16x2(hi, w), lo = first && i == 0 ? w : min_bf16x2(lo, w);
+  }
+}
+DEVI void extremes_of(uint32_t hi, uint32_t lo, float& mn, float& mx) {
+  // a NaN in either half has to come through
+  const uint32_t m = max_bf16x2(hi, hi >> 16 | hi << 16), n = min_bf16x2(lo, lo >> 16 | lo << 16);
+  mx = bf16_lo(m), mn = bf16_lo(n);
+}
+// ... and with the clamp, where that is needed
+DEVI void extremes_32_clamped(const float* v, float& mn, float& mx) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
     const float x = kv4_clamp(__bfloat162float(__float2bfloat16_rn(v[i])));
     mn = fminf(mn, x), mx = fmaxf(mx, x);
   }
-  const Kv4Group g = kv4_group(mn, mx);
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      w[i >> 3] |= (uint32_t)kv4_code(kv4_clamp(__bfloat162float(__float2bfloat16_rn(v[32 * c + i]))), g) << ((i & 7) * 4);
-    *reinterpret_cast<uint4*>(codes + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  *pair = g.word;
 }
-
-// The same for 32 values already rounded to bf16, whose vector's or group's scale is known.
+// the codes of 32 values of a group; tame: its values need no clamp
+DEVI void store_q4_32(const float* v, const Kv4Group& g, bool tame, uint8_t* codes) {
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (tame && kv4_plain(g)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const uint32_t b = pack_bf16(v[8 * c + i], v[8 * c + i + 1]);
+        x[i] = bf16_lo(b), x[i + 1] = bf16_hi(b);
+      }
+      w[c] = kv4_codes8<true>(x, g);
+    }
+  } else {
+    float x[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = __bfloat162float(__float2bfloat16_rn(v[i]));
+    kv4_codes_slow<32, true>(x, g, w);
+  }
+  *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+// int8 for 32 values already rounded to bf16, whose vector's scale is known.
 DEVI void store_q8_32(const float (&f)[32], float inv, int8_t* dst) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -53,11 +76,4 @@ DEVI void store_q8_32(const float (&f)[32], float inv, int8_t* dst) {
     *reinterpret_cast<uint4*>(dst + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-DEVI void store_q4_32(const float (&f)[32], const Kv4Group& g, uint8_t* codes) {
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 32; ++i) w[i >> 3] |= (uint32_t)kv4_code(kv4_clamp(f[i]), g) << ((i & 7) * 4);
-  *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 }  // namespace b200dec_detail

@@ -196,6 +196,46 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArg
       }
       for (int c0 = 0; c0 < TN; c0 += 64) {  // warp-uniform trip count: the tensor-memory loads are collective
         const int n0 = nt * TN + c0;
+        // channel n0 = ((layer * 2 + k|v) * H + head) * D + d
+        if (p.mode == 3) {  // 64 channels are one group of the 4-bit format: 32 at a time, for their extremes and to be stored
+          const auto load32 = [&](int c, float (&f)[32]) {
+            uint32_t e[32];
+            __syncwarp();  // a collective load: rows without a slot may have gone ahead
+            tmem_ld32(acc + c0 + c, e);
+            tmem_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(e[i]);
+            if (p.bias) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + n0 + c) + i);
+                f[4 * i] += b.x, f[4 * i + 1] += b.y, f[4 * i + 2] += b.z, f[4 * i + 3] += b.w;
+              }
+            }
+          };
+          const int hd = p.H * p.D, l = n0 / (2 * hd), kvi = (n0 / hd) & 1, h = (n0 % hd) / p.D, d0 = n0 % p.D;
+          const size_t at = (slot < 0 ? 0 : ((((size_t)l * p.S1 + slot) * p.H + h) * p.T + frame) * p.D) + d0;
+          float f[32], mn, mx;
+          uint32_t hi = 0, lo = 0;
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 32) load32(c, f), extremes_32(f, c == 0, hi, lo);
+          extremes_of(hi, lo, mn, mx);
+          const bool tame = kv4_tame(mn, mx);
+          if (__any_sync(0xffffffffu, !tame)) {
+            mn = INFINITY, mx = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 32) load32(c, f), extremes_32_clamped(f, mn, mx);
+          }
+          const Kv4Group g = kv4_group(mn, mx);
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 32) {
+            load32(c, f);
+            if (slot >= 0) store_q4_32(f, g, tame, reinterpret_cast<uint8_t*>(kvi ? p.cv : p.ck) + (at + c) / 2);
+          }
+          if (slot >= 0) reinterpret_cast<uint32_t*>(kvi ? p.cvs : p.cks)[at / 64] = g.word;
+          __syncwarp();
+          continue;
+        }
         float v[64];
         tmem_ld64(acc + c0, v);
         if (p.bias) {
@@ -222,10 +262,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefill_gemm_kernel(const GemmArg
                   make_uint4(pack_bf16(v[8 * c], v[8 * c + 1]), pack_bf16(v[8 * c + 2], v[8 * c + 3]),
                              pack_bf16(v[8 * c + 4], v[8 * c + 5]), pack_bf16(v[8 * c + 6], v[8 * c + 7]));
           }
-        } else if (p.mode == 3) {  // 64 channels are one group of the 4-bit format
-          if (slot >= 0)
-            store_q4_64(v, reinterpret_cast<uint8_t*>(kvi ? p.cv : p.ck) + (vec * p.D + d0) / 2,
-                        reinterpret_cast<uint32_t*>(kvi ? p.cvs : p.cks) + (vec * p.D + d0) / 64);
         } else if constexpr (TN == BN) {
           // int8: the vector's absmax over its D = 64 or 128 channels after rounding to bf16
           float mx = 0.f;

@@ -353,19 +353,33 @@ __global__ void __launch_bounds__(NTHREADS, 1) w8a8_kernel(const W8Args p) {
           const int n = n0 + c, hd = p.H * p.D, l = n / (2 * hd), kvi = (n / hd) & 1, h = (n % hd) / p.D, d0 = n % p.D;
           const size_t vec = slot < 0 ? 0 : ((((size_t)l * p.S1 + slot) * p.H + h) * p.T + frame);
           char* cache = reinterpret_cast<char*>(kvi ? p.cv : p.ck);
-          float mn = INFINITY, mx = -INFINITY;
+          float mn = 0.f, mx = 0.f;
+          bool tame = true;
           if (p.mode != 1) {
+            uint32_t hi = 0, lo = 0;
 #pragma unroll 1
             for (int i = 0; i < span; i += 32) {
               load(c + i, v, B200DEC_ACT_NONE);
+              if (p.mode == 3) extremes_32(v, i == 0, hi, lo);
+              else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const float b = __bfloat162float(__float2bfloat16_rn(v[j])), x = p.mode == 3 ? kv4_clamp(b) : b;
-                mn = fminf(mn, x), mx = fmaxf(mx, x);
+                for (int j = 0; j < 32; ++j) mx = fmaxf(mx, fabsf(__bfloat162float(__float2bfloat16_rn(v[j]))));
+              }
+            }
+            if (p.mode == 3) {
+              extremes_of(hi, lo, mn, mx);
+              tame = kv4_tame(mn, mx);
+              if (__any_sync(0xffffffffu, !tame)) {  // some row of the warp: all of them again, the loads are the warp's
+                mn = INFINITY, mx = -INFINITY;
+#pragma unroll 1
+                for (int i = 0; i < span; i += 32) {
+                  load(c + i, v, B200DEC_ACT_NONE);
+                  extremes_32_clamped(v, mn, mx);
+                }
               }
             }
           }
-          const float top = fmaxf(fmaxf(mx, -mn), 0.f), s8 = top > 0.f ? __fdiv_rn(top, 127.f) : 1.f, inv8 = __fdiv_rn(1.f, s8);
+          const float s8 = p.mode == 2 && mx > 0.f ? __fdiv_rn(mx, 127.f) : 1.f, inv8 = __fdiv_rn(1.f, s8);
           const Kv4Group g = kv4_group(mn, mx);
 #pragma unroll 1
           for (int i = 0; i < span; i += 32) {
@@ -377,11 +391,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) w8a8_kernel(const W8Args p) {
                 for (int j = 0; j < 32; j += 8)
                   *reinterpret_cast<uint4*>(cache + (at + j) * 2) = make_uint4(pack_bf16(v[j], v[j + 1]), pack_bf16(v[j + 2], v[j + 3]),
                                                                                pack_bf16(v[j + 4], v[j + 5]), pack_bf16(v[j + 6], v[j + 7]));
-              } else {
+              } else if (p.mode == 2) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
-                if (p.mode == 2) store_q8_32(v, inv8, reinterpret_cast<int8_t*>(cache) + at);
-                else store_q4_32(v, g, reinterpret_cast<uint8_t*>(cache) + at / 2);
+                store_q8_32(v, inv8, reinterpret_cast<int8_t*>(cache) + at);
+              } else {
+                store_q4_32(v, g, tame, reinterpret_cast<uint8_t*>(cache) + at / 2);
               }
             }
           }
