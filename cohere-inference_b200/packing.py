@@ -215,6 +215,8 @@ class W8A8Linear:
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None, act: str | None = None):
         if not (q.is_cuda and q.dtype == torch.int8 and q.dim() == 2 and q.numel()):
             raise ValueError("W8A8Linear: q must be a non-empty int8 (n, k) matrix on a CUDA device")
+        if act not in self.ACTS:
+            raise ValueError(f"W8A8Linear: act is one of {tuple(self.ACTS)}")
         self.n, self.k, self.device, self.act = int(q.shape[0]), int(q.shape[1]), q.device, self.ACTS[act]
         if scale.shape != (self.n,) or (bias is not None and bias.shape != (self.n,)):
             raise ValueError("W8A8Linear: one scale (and bias) per channel")

@@ -276,6 +276,56 @@ def test_attention_q4_peaked_and_tiny_weights(nv):
     assert torch.allclose(out.double(), ref, rtol=2e-4, atol=64 * 2.0 ** -32)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("self", [True, False])
+def test_attention_q4_awkward_vectors(nv, self, dim):
+    """Constant, zero, tiny and far-off vectors among the cached ones and as the new key and value: pairs with step 0, groups of a
+    key with unlike steps, and nothing but constants in a whole row."""
+    heads, cap, rows = 2, 150, 3
+    x = awkward_rows(2 * (rows + 1) * cap, heads * dim, 21).view(2, rows + 1, cap, heads, dim).transpose(2, 3)
+    x = torch.nan_to_num(x, 0.0, 2.0, -2.0).clamp(-1000, 1000)
+    x[:, 1] = x[:, 1, :, :1, :1]  # slot 1: every vector of a head the same constant
+    (k, km, _), (v, vm, _) = quantise(x[0]), quantise(x[1])
+    active = torch.tensor([2, 1, 0], dtype=torch.int32, device="cuda")
+    n = torch.tensor([149, 140, 37, 1], dtype=torch.int32, device="cuda")
+    q = 0.01 * torch.randn(rows, (3 if self else 1) * heads * dim, generator=gen(22), device="cuda")
+    if self:
+        q[0, heads * dim:] = 0.25  # a constant key and value
+    caches = k, v, km, vm
+    ref, far = reference(self, active, q, caches, n, heads, dim)
+    out = torch.empty(rows, heads * dim, device="cuda")
+    assert attend(nv, self, active, q, caches, n, rows, heads, dim, cap, out) == 0
+    check(out, ref, far)
+
+
+def test_far_offsets_in_4_bit_caches(nv):
+    """A cache whose last slots lie beyond 2^32 bytes: filled, appended to, attended and read back there."""
+    slots, heads, cap, dim, n = 41, 16, 220000, 64, 333
+    shape = 1, slots + 1, heads, cap
+    k, v = (torch.zeros(*shape, dim // 2, dtype=torch.uint8, device="cuda") for _ in range(2))
+    km, vm = (torch.zeros(*shape, 1, 2, dtype=torch.float16, device="cuda") for _ in range(2))
+    assert slots * heads * cap * dim // 2 > 2 ** 32
+    kv = torch.randn(n, 2 * heads * dim, generator=gen(30), device="cuda")
+    slot_of = torch.full((n,), slots - 1, dtype=torch.int32, device="cuda")
+    frame_of = torch.arange(n, dtype=torch.int32, device="cuda")
+    p, sizes = nv.ptr, (1, slots + 1, heads, dim, cap, nv.stream_ptr())
+    nv.check(nv.lib().b200dec_scatter_kv_q4(p(kv), p(slot_of), p(frame_of), p(k), p(v), p(km), p(vm), n, *sizes))
+    active = slot_of[:1].contiguous()
+    lens = torch.zeros(slots + 1, dtype=torch.int32, device="cuda")
+    lens[slots - 1] = n
+    q = torch.randn(1, 3 * heads * dim, generator=gen(31), device="cuda")
+    caches = k[0], v[0], km[0], vm[0]
+    ref, far = reference(True, active, q, caches, lens, heads, dim)
+    out = torch.empty(1, heads * dim, device="cuda")
+    assert attend(nv, True, active, q, caches, lens, slots, heads, dim, cap, out) == 0
+    check(out, ref, far)
+    rows = torch.cat((kv, q[:, heads * dim:]))
+    slot_of, frame_of = torch.full((n + 1,), slots - 1, dtype=torch.int32, device="cuda"), torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    back = torch.empty_like(rows)
+    nv.check(nv.lib().b200dec_gather_kv_q4(p(back), p(slot_of), p(frame_of), p(k), p(v), p(km), p(vm), n + 1, *sizes))
+    assert torch.equal(back, quantise(rows.view(n + 1, -1, dim))[2].flatten(1).float())
+
+
 def test_attention_q4_out_of_range(nv):
     """Lengths and slots outside the tables are clamped and reported; the neighbours are right all the same."""
     heads, dim, cap, slots = 2, 64, 40, 3
@@ -511,6 +561,26 @@ def test_logit_rules_corners(nv):
     assert int(pick[0]) == int((x == x.max()).nonzero()[0])
 
 
+def test_logit_rules_far_offsets(nv):
+    """Rows beyond 2^32 elements, a vocabulary of 2^24 that no CTA marks in one go, and tokens in its last places."""
+    rows, vocab, slots = 258, 1 << 24, 258
+    logits = torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    assert (rows - 1) * vocab > 2 ** 32 - 1
+    t = tables(slots, vocab, 20, 2, 3)
+    t["last"][:], t["plen"][:], t["bias_n"][:] = 19, 0, 0
+    t["params"][:] = torch.tensor([1.0, 0.0, 0.5, 0.0], device="cuda")
+    last = rows - 1
+    t["history"][last] = vocab - 5
+    logits[last, vocab - 5] = 9.0   # taken 20 times: 9 - 10
+    logits[last, vocab - 3] = 3.0
+    logits[last, 7] = 2.0
+    logits[0, 1 << 23] = 1.0
+    active = torch.arange(rows, dtype=torch.int32, device="cuda")
+    token, best, status = run_rules(nv, logits, vocab, active, slots, rules_of(nv, t, mask=False))
+    assert int(token[last]) == vocab - 3 and float(best[last]) == 3.0
+    assert int(token[0]) == 1 << 23 and float(best[0]) == 1.0 and status == 0
+
+
 # ---- the 8-bit product ------------------------------------------------------------------------------------------------------
 
 
@@ -553,6 +623,21 @@ def test_w8a8_linear(nv, m, k, n, x_type, out_type):
         worst = ((y.double() - ref).abs() - far).max()
         assert y.dtype == out_type and worst <= 0, float(worst)
         assert int(lin.status) == 0
+
+
+def test_w8a8_far_offsets(nv):
+    """Results beyond 2^32 bytes."""
+    from cohere_inference_b200.packing import W8A8Linear
+    g = gen(40)
+    m, k, n = 70001, 64, 16400
+    x = torch.randn(m, k, generator=g, device="cuda", dtype=torch.float32)
+    q = torch.randint(-127, 128, (n, k), generator=g, device="cuda").to(torch.int8)
+    scale = torch.rand(n, generator=g, device="cuda") * 0.01
+    y = W8A8Linear(q, scale)(x)
+    assert (m - 1) * n * 4 > 2 ** 32
+    for rows in (slice(0, 3), slice(m // 2, m // 2 + 3), slice(m - 3, m)):
+        ref, size = product(x[rows], q, scale, None, None)
+        assert ((y[rows].double() - ref).abs() <= 5 * HALF[torch.float32] * size).all()
 
 
 def test_w8a8_quantises_as_if_exact(nv):
@@ -638,7 +723,7 @@ def test_w8a8_refusals(nv):
             lin(x, out=bad)
     with pytest.raises(ValueError):
         lin(x, out=torch.empty(3, 8, device="cuda"), dtype=torch.float16)
-    for args in ((q.cpu(), s), (q.float(), s), (q[:0], s[:0]), (q, s[:7]), (q, s, torch.ones(7, device="cuda")),
+    for args in ((q, s, None, "tanh"), (q.cpu(), s), (q.float(), s), (q[:0], s[:0]), (q, s[:7]), (q, s, torch.ones(7, device="cuda")),
                  (torch.ones(1, 131073, dtype=torch.int8, device="cuda"), s[:1])):
         with pytest.raises(ValueError):
             W8A8Linear(*args)
