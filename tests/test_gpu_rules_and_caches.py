@@ -107,6 +107,32 @@ def test_steps_over_4_bit_caches(model16, heads, mode):
         assert ((got - full.double()).abs() <= half * 1.01 + 2.0 ** -8 * full.abs().double() + 2.0 ** -11 * want.abs()).all()
 
 
+@pytest.mark.parametrize("heads", [16, 8])
+@pytest.mark.parametrize("rows", [5, 40])
+def test_steps_over_4_bit_caches_do_not_depend_on_how_they_are_launched(model16, heads, rows):
+    """Graphs of programmatic launches against plain launches, one kernel fully before the next: the same bits for 60 steps, so
+    no step reads a key or a pair from before it was written."""
+    model = model16 if heads == 16 else synthetic_model(3, heads=8, head_dim=128, act="relu")
+    rng = np.random.default_rng(9)
+    frames = rng.integers(20, 300, rows).tolist()
+    memory = torch.randn(sum(frames), 1024, generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    prompts, slots = [rng.integers(0, 16384, 5) for _ in range(rows)], list(range(rows))
+    got = []
+    for kw in (dict(), dict(pdl=0, graphs=False)):
+        dec = decoder(model, slots=48, max_new_tokens=70, int8=True, kv_int4=True, record=True, **kw)
+        with torch.cuda.stream(dec.stream):
+            dec.fill_cross(memory, frames, slots)
+        dec.admit(slots, prompts, frames)
+        b = dec.set_active(slots)
+        for _ in range(60):
+            dec.step(b)
+        dec.stream.synchronize()
+        dec.check_status()
+        got.append((dec.out[:rows].clone(), dec.logits[:rows].clone(), dec.self_k.clone(), dec.self_vs.clone()))
+    for x, y in zip(*got):
+        assert torch.equal(x[:, :rows] if x.dim() > 2 else x, y[:, :rows] if y.dim() > 2 else y)
+
+
 def test_4_bit_caches_stay_near_the_oracle(model16):
     """Logits over 4-bit caches against the bf16-cache decoder on the same tokens. A cached value is off by at most half a
     step, a fifteenth of its group's range / 2, that is about 0.1 of its spread, at random: with 50 keys and more an
