@@ -32,6 +32,7 @@ constexpr int MAX_BIAS = 1024, MAX_CLUSTER = 8, NONE = 0x7fffffff, NT = 512, CTA
 constexpr int RING = 4;
 constexpr int SMEM_BUDGET = 100 * 1024;  // of a CTA: two per SM
 constexpr int SMEM_RING = RING * NT * 16;
+constexpr int SMEM_STATIC = (2 * MAX_CLUSTER + 3 * (NT / 32)) * 4;  // the kernel's own arrays: the row's and its warps' best, the warps' sums
 
 static_assert(MAX_BIAS <= 2 * NT, "a thread stages two biases");
 
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(NT, CTAS_PER_SM) logit_rules_kernel(const Rule
 template <int KIND>
 cudaError_t launch_rules(const RulesArgs& p, int rows, int cluster, int nb, cudaStream_t st, int pdl) {
   const size_t smem = SMEM_RING + (size_t)p.tile / 4 + (size_t)p.dense * 4 + (size_t)nb * 8;
-  if (smem > 48 * 1024) {
+  if (smem + SMEM_STATIC > 48 * 1024) {  // what a CTA has unasked holds the static arrays too
     const cudaError_t e = cudaFuncSetAttribute(logit_rules_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BUDGET);
     if (e != cudaSuccess) return e;
   }
