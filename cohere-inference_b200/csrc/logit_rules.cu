@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(NT, CTAS_PER_SM) logit_rules_kernel(const Rule
   const uint32_t* mask = p.r.mask && (!p.r.mask_on || p.r.mask_on[s]) ? p.r.mask + (size_t)s * ((p.vocab + 31) / 32) : nullptr;
   const float rep = par.x, presence = par.y, frequency = par.z;
   const bool penal = rep != 1.f || presence != 0.f || frequency != 0.f;
-  const int have = penal ? min(newest, p.r.hist_cols - 1) + 1 : 0;  // tokens that count
+  const int have = penal ? min(max(newest, -1), p.r.hist_cols - 1) + 1 : 0;  // tokens that count
   const bool touched = have > 0 || nb > 0;
   float* b_val = reinterpret_cast<float*>(b_id + nb);
   // The first logits come in while the slot's tokens are counted: two vectors behind the loads of its tables, the others when

@@ -89,7 +89,7 @@ typedef struct b200dec_rules {
   const float* params;     /* (slots + 1, 4), 16-byte aligned: repetition penalty (> 0; 1: none), presence penalty, frequency
                               penalty (0: none), unused */
   const int64_t* history;  /* (slots + 1, hist_cols): the slot's tokens; ids outside the vocabulary count for nothing */
-  const int32_t* last;     /* (slots + 1): history[0 .. last] counts (-1: none), last < hist_cols */
+  const int32_t* last;     /* (slots + 1): history[0 .. last] counts (-1 and below: none), up to hist_cols tokens */
   const int32_t* plen;     /* (slots + 1): history[plen .. last] are generated, what is before them is the prompt */
   const int32_t* bias_ids; /* NULL (with the next two), or (slots + 1, max_bias) token ids, */
   const float* bias;       /* what is added to their logits (-INFINITY bans a token; one listed twice gets both), */

@@ -1,4 +1,4 @@
-"""Edges of the rules on the logits: sizes of shared memory around the limit that needs no opt-in."""
+"""Edges of the rules on the logits: sizes of shared memory around the limit that needs no opt-in, slots without tokens."""
 
 import math
 import os
@@ -16,6 +16,13 @@ from test_gpu_operators import gen, rules_of, run_rules, tables, under_rules  # 
 from test_gpu_rules_and_caches import decoder, start  # noqa: E402
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def nv():
+    from cohere_inference_b200 import native
+    native.lib()
+    return native
 
 
 def in_a_fresh_process(call):
@@ -55,3 +62,23 @@ def most_biases():
 
 def test_decoder_with_the_most_biases():
     in_a_fresh_process("most_biases()")
+
+
+@pytest.mark.parametrize("last", [-1, -2, -9, -(1 << 31)])
+def test_logit_rules_of_a_slot_without_tokens(nv, last):
+    """Below -1 is no token, as -1 is: every listed bias counts, every logit is written."""
+    rows, vocab, slots, n = 3, 5000, 3, 12
+    t = tables(slots, vocab, 40, n, 31)
+    t["last"][:], t["bias_n"][:] = -1, n
+    t["params"][:, :3] = torch.tensor([2.0, 1.0, 0.5], device="cuda")
+    t["mask_on"][:] = torch.tensor([0, 1, 0, 0], device="cuda")
+    active = torch.arange(rows, dtype=torch.int32, device="cuda")
+    logits = ((torch.randn(rows, vocab, generator=gen(32), device="cuda") * 16).round() / 8).clamp(-12, 12)
+    want = [under_rules(logits[r], r, t) for r in range(rows)]
+    t["last"][:] = last
+    out = torch.full((rows, vocab), 77.0, device="cuda")
+    token, best, status = run_rules(nv, logits, vocab, active, slots, rules_of(nv, t), out, vocab)
+    for r, x in enumerate(want):
+        assert int(token[r]) == int((x == x.max()).nonzero()[0]) and float(best[r]) == float(x.max())
+        assert torch.equal(out[r].double(), x)
+    assert status == 0
