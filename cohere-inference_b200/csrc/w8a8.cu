@@ -70,8 +70,13 @@ DEVI void umma_i8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uin
 }
 DEVI void epi_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory"); }
 
+DEVI float relu(float x) {  // NaN stays NaN (fmaxf would make it 0)
+  float y;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+  return y;
+}
 DEVI float activate(float x, int act) {
-  if (act == B200DEC_ACT_RELU) return fmaxf(x, 0.f);
+  if (act == B200DEC_ACT_RELU) return relu(x);
   if (act == B200DEC_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
   return x;
 }

@@ -1,4 +1,5 @@
-"""Edges of the rules on the logits: sizes of shared memory around the limit that needs no opt-in, slots without tokens."""
+"""Edges of the rules on the logits and of the 8-bit product: sizes of shared memory around the limit that needs no opt-in, slots without
+tokens, NaN through the activations."""
 
 import math
 import os
@@ -82,3 +83,21 @@ def test_logit_rules_of_a_slot_without_tokens(nv, last):
         assert int(token[r]) == int((x == x.max()).nonzero()[0]) and float(best[r]) == float(x.max())
         assert torch.equal(out[r].double(), x)
     assert status == 0
+
+
+@pytest.mark.parametrize("act", [None, "relu", "gelu"])
+@pytest.mark.parametrize("out_type", [torch.float32, torch.float16, torch.bfloat16])
+def test_w8a8_bad_rows_stay_bad(act, out_type):
+    """A row with an infinity or NaN gives NaN, whatever the activation; the others what they give alone."""
+    from cohere_inference_b200.packing import W8A8Linear
+    g = gen(2)
+    m, k, n = 70, 200, 90
+    lin = W8A8Linear.from_weight(torch.randn(n, k, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda"), act)
+    x = torch.randn(m, k, generator=g, device="cuda")
+    clean = lin(x, dtype=out_type)
+    x[4, 9], x[5, 0], x[6, k - 1] = math.nan, math.inf, -math.inf
+    y = lin(x, dtype=out_type)
+    assert y[4:7].isnan().all()
+    rest = torch.arange(m, device="cuda")
+    rest = rest[(rest < 4) | (rest > 6)]
+    assert torch.equal(y[rest], clean[rest]) and (act != "relu" or (clean >= 0).all())
