@@ -45,6 +45,7 @@ struct RulesArgs {
   float* best;
   int* token;
   int* status;
+  const uint8_t* finished;  // null: every row's choice is taken; else (slots + 1): not that of a row that has ended or is fed its prompt
   int vocab, slots, range;  // range: positions of a CTA, a multiple of 32
   int tile, dense;          // positions marked at a time, a multiple of 32, and the words of their table
 };
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(NT, CTAS_PER_SM) logit_rules_kernel(const Rule
     for (int i = 0; i < ranks; ++i) all.take(s_best[i], s_arg[i]);
     if (all.i == NONE) {  // nothing above -inf: the first token, and said so
       all.i = 0;
-      if (s < p.slots) atomicOr(p.status, B200DEC_ST_NO_TOKEN);
+      if (s < p.slots && (!p.finished || (!p.finished[s] && p.r.last[s] + 1 >= p.r.plen[s]))) atomicOr(p.status, B200DEC_ST_NO_TOKEN);
     }
     p.token[row] = all.i;
     if (p.best) p.best[row] = all.v;
@@ -383,8 +384,8 @@ cudaError_t launch_rules(const RulesArgs& p, int rows, int cluster, int nb, cuda
 namespace b200dec_detail {
 
 int logit_rules_impl(const void* logits, int kind, int64_t ldl, int rows, int vocab, const int32_t* active, int slots,
-                     const b200dec_rules* rules, void* out, int64_t ldo, float* best, int32_t* token, int32_t* status, int pdl,
-                     void* stream) {
+                     const b200dec_rules* rules, void* out, int64_t ldo, float* best, int32_t* token, int32_t* status,
+                     const uint8_t* finished, int pdl, void* stream) {
   B200_REQUIRE(logits && active && rules && token && status, "logit_rules: null pointer");
   B200_REQUIRE(kind == B200DEC_T_F32 || kind == B200DEC_T_F16 || kind == B200DEC_T_BF16, "logit_rules: kind %d", kind);
   B200_REQUIRE(rows >= 1 && rows <= 65535 && vocab >= 1 && vocab <= 1 << 24 && slots >= 0 && ldl >= vocab && (!out || ldo >= vocab),
@@ -402,7 +403,7 @@ int logit_rules_impl(const void* logits, int kind, int64_t ldl, int rows, int vo
   // row, 38 with two (this rule), 41 with three, 43 with four
   int cluster = 1;
   while (cluster < MAX_CLUSTER && rows * cluster * 2 <= CTAS_PER_SM * 148 * 9 / 10 && vocab / (cluster * 2) >= 2048) cluster *= 2;
-  RulesArgs p{logits, out, ldl, ldo, active, *rules, best, token, status, vocab, slots, 0, 0, 0};
+  RulesArgs p{logits, out, ldl, ldo, active, *rules, best, token, status, finished, vocab, slots, 0, 0, 0};
   p.range = ((vocab + 7 + cluster - 1) / cluster + 31) / 32 * 32;  // of vocab + pad positions
   // a position takes 8 / 32 bytes of marks and counts, a marked one a word: no more of those than tokens and biases, or positions
   const int nb = rules->bias_ids ? rules->max_bias : 0;
@@ -424,5 +425,5 @@ int logit_rules_impl(const void* logits, int kind, int64_t ldl, int rows, int vo
 extern "C" int b200dec_logit_rules(const void* logits, int kind, int64_t ldl, int rows, int vocab, const int32_t* active, int slots,
                                    const b200dec_rules* rules, void* out, int64_t ldo, float* best, int32_t* token,
                                    int32_t* status, int pdl, void* stream) {
-  return logit_rules_impl(logits, kind, ldl, rows, vocab, active, slots, rules, out, ldo, best, token, status, pdl, stream);
+  return logit_rules_impl(logits, kind, ldl, rows, vocab, active, slots, rules, out, ldo, best, token, status, nullptr, pdl, stream);
 }

@@ -28,8 +28,8 @@ int attention_spans_impl(int self, const int32_t* sched, const float* q, int ldq
                          float* vscale, int heads, int head_dim, int cap, float scale, void* out, int out_kind, int rows,
                          int64_t step_items, int pdl, void* stream);
 int logit_rules_impl(const void* logits, int kind, int64_t ldl, int rows, int vocab, const int32_t* active, int slots,
-                     const b200dec_rules* rules, void* out, int64_t ldo, float* best, int32_t* token, int32_t* status, int pdl,
-                     void* stream);
+                     const b200dec_rules* rules, void* out, int64_t ldo, float* best, int32_t* token, int32_t* status,
+                     const uint8_t* finished, int pdl, void* stream);
 bool fused_step_applies(const b200dec_plan* pl, int row0, int rows);
 int fused_step(const b200dec_plan* pl, int rows, void* stream);
 }  // namespace b200dec_detail
@@ -285,7 +285,7 @@ int b200dec_step_part(const b200dec_plan* pl, int row0, int rows, int step_rows,
   const int32_t* pick_idx = head_idx;
   if (pl->rules) {
     B200_TRY_IN(1, logit_rules_impl(logits, B200DEC_T_F32, pl->vocab, rows, pl->vocab, active, pl->slots, pl->rules, nullptr, 0,
-                                    pl->rule_best + row0, pl->rule_token + row0, pl->status, pdl, stream));
+                                    pl->rule_best + row0, pl->rule_token + row0, pl->status, pl->finished, pdl, stream));
     pick_max = pl->rule_best + row0, pick_idx = pl->rule_token + row0;
   }
   B200_TRY_IN(1, pick_impl(pick_max, pick_idx, pl->rules ? 1 : partials, active, rows, pl->slots, pl->tok, pl->pos, pl->finished, pl->forced,

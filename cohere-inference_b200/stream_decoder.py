@@ -805,7 +805,8 @@ class StreamDecoder:
         """What the next steps of these slots may choose: per slot None (everything), booleans over the vocabulary (True =
         allowed), or the mask's 32-bit words (bit v % 32 of word v / 32); holds until it is set again or the slot admits
         another request. A grammar sets it between steps. On the decoder stream, so it counts from the next step
-        launched. A mask that allows nothing makes the choice token 0 and is reported by check_status."""
+        launched. A mask that allows nothing makes the choice token 0, which check_status reports where the choice is taken (not
+        while the prompt is fed, nor after the row has ended)."""
         if not self.logit_rules or len(masks) != len(slots) or not all(0 <= s < self.slots for s in slots):
             raise ValueError(f"set_mask: one mask per slot (0..{self.slots - 1}), in a decoder made with logit_rules=True")
         words = (self.vocab + 31) // 32

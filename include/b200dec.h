@@ -170,7 +170,8 @@ typedef struct b200dec_plan {
   /* kv_int4 != 0: 4-bit caches (see b200dec_attention_q4); the layers' caches hold codes, self_ks .. cross_vs their fp16 pairs.
    * rules: NULL, or the rules the choice goes by (a host struct of device tables): the step then writes its logits, b200dec_logit_rules
    * takes them into rule_best / rule_token (max rows each), and the pick chooses from those; `logits` must be there and keeps
-   * the logits before the rules. Steps with either are not fused. */
+   * the logits before the rules; B200DEC_ST_NO_TOKEN is raised only for rows that take their choice, not for those that are fed
+   * their prompt or have ended. Steps with either are not fused. */
   int32_t kv_int4, _pad2;
   const b200dec_rules* rules;
   float* rule_best;

@@ -1,11 +1,12 @@
 """Edges of the rules on the logits and of the 8-bit product: sizes of shared memory around the limit that needs no opt-in, slots without
-tokens, NaN through the activations."""
+tokens, NaN through the activations, rows whose choice nobody takes."""
 
 import math
 import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 import torch
 
@@ -24,6 +25,11 @@ def nv():
     from cohere_inference_b200 import native
     native.lib()
     return native
+
+
+@pytest.fixture(scope="module")
+def model16():
+    return synthetic_model(0)
 
 
 def in_a_fresh_process(call):
@@ -101,3 +107,33 @@ def test_w8a8_bad_rows_stay_bad(act, out_type):
     rest = torch.arange(m, device="cuda")
     rest = rest[(rest < 4) | (rest > 6)]
     assert torch.equal(y[rest], clean[rest]) and (act != "relu" or (clean >= 0).all())
+
+
+NOTHING = np.zeros(16384, bool)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(chains=2, slots=16, buckets=(16,)), dict(graphs=False, pdl=0)])
+def test_only_choices_that_are_taken_are_reported(model16, kw):
+    """A mask that allows nothing is no mistake of a row whose prompt is still fed, nor of one that has ended; it is one as soon as
+    the row's choice is taken."""
+    from cohere_inference_b200.native import NativeError
+    dec = decoder(model16, int8=True, logit_rules=True, **kw)
+    frames, memory, prompts = [60, 60], torch.randn(120, 1024, device="cuda"), [np.arange(1, 11), np.arange(3, 5)]
+    with torch.cuda.stream(dec.stream):
+        dec.stream.wait_stream(torch.cuda.default_stream())
+        dec.fill_cross(memory, frames, [1, 6])
+    dec.admit([1, 6], prompts, frames, max_new=[48, 3], rules=[dict(mask=NOTHING), None])
+    b = dec.set_active([1, 6])
+    for _ in range(4):  # the second: one step of its prompt, then the three tokens of its budget
+        dec.step(b)
+    dec.check_status()
+    assert int(dec.finished[6]) == 1
+    dec.set_mask([6], [NOTHING])
+    for _ in range(5):  # the first: positions 5 to 9 of its prompt
+        dec.step(b)
+    dec.check_status()
+    assert int(dec.pos[1]) == 9 and int(dec.tok[1]) == 10
+    dec.step(b)
+    with pytest.raises(NativeError, match="left no token"):
+        dec.check_status()
+    assert int(dec.tok[1]) == 0
