@@ -207,7 +207,8 @@ class W8A8Linear:
     quantised as they come, one scale each. The form for many rows (encoder frames, whole sentences); the decoding step's
     projections keep 16-bit rows (PackedLinear). q: int8 (n, k) and scale: fp32 (n,) as quantize_rows gives them, bias: (n,)
     or None. Holds its own copies; a call allocates what it needs on the current stream, so calls on several streams and
-    inside a capture are like any other torch operation's."""
+    inside a capture are like any other torch operation's. Calls and replays do not wait for their results, so a wait inside the
+    kernel that ran out (every one is bounded) shows in check_status: ask it before results are given away."""
 
     ACTS = {None: nv.ACT_NONE, "relu": nv.ACT_RELU, "gelu": nv.ACT_GELU}
     KINDS = {torch.float32: nv.T_F32, torch.float16: nv.T_F16, torch.bfloat16: nv.T_BF16}
@@ -265,6 +266,18 @@ class W8A8Linear:
             with torch.cuda.device(dev):
                 return self._run(x, x_kind, m, ldx, out, kind, ldo)
         return self._run(x, x_kind, m, ldx, out, kind, ldo)
+
+    def check_status(self) -> None:
+        """Waits for the device, and raises if a bounded wait inside a kernel ran out in any call or replay since the last check:
+        rows of such a call's result were not written. The word is cleared, so that later calls are judged by themselves."""
+        if self.status.is_cuda:
+            torch.cuda.synchronize(self.status.device)
+        st = int(self.status.item())
+        if st:
+            self.status.zero_()
+            if self.status.is_cuda:
+                torch.cuda.synchronize(self.status.device)  # no later call, on whatever stream, has its bit wiped out
+            raise nv.NativeError(f"W8A8Linear: a bounded wait inside a kernel ran out (status {st}): results are incomplete")
 
     def _run(self, x, x_kind, m, ldx, out, kind, ldo) -> torch.Tensor:
         lib, k = nv.lib(), self.k

@@ -137,3 +137,18 @@ def test_only_choices_that_are_taken_are_reported(model16, kw):
     with pytest.raises(NativeError, match="left no token"):
         dec.check_status()
     assert int(dec.tok[1]) == 0
+
+
+def test_w8a8_check_status(nv):
+    """Nothing to report after calls; a word set on the device (as a wait that runs out sets it) is reported and cleared."""
+    from cohere_inference_b200.packing import W8A8Linear
+    lin = W8A8Linear(torch.eye(64, dtype=torch.int8, device="cuda"), torch.ones(64, device="cuda"))
+    x = torch.randn(5, 64, device="cuda")
+    y = lin(x)
+    lin.check_status()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        lin.status.fill_(nv.ST_TIMEOUT)
+        with pytest.raises(nv.NativeError, match="ran out"):
+            lin.check_status()
+    assert torch.equal(lin(x), y)
+    lin.check_status()
