@@ -769,12 +769,16 @@ class StreamDecoder:
             r = r or {}
             unknown = set(r) - {"repetition", "presence", "frequency", "bias", "mask"}
             bias = dict(r.get("bias") or {})
-            pens = [float(r.get(k, d)) for k, d in (("repetition", 1.0), ("presence", 0.0), ("frequency", 0.0))]
+            with np.errstate(over="ignore"):  # judged as the fp32 numbers that the kernel reads: 1e-50 is 0 there, 1e39 infinite
+                pens = np.array([float(r.get(k, d)) for k, d in (("repetition", 1.0), ("presence", 0.0), ("frequency", 0.0))]).astype(np.float32)
             if unknown or len(bias) > nb or not np.all(np.isfinite(pens)) or pens[0] <= 0:
                 raise ValueError(f"admit: rules {sorted(unknown) or pens} with {len(bias)} biases (at most {nb}; repetition > 0)")
             ids, vals = [int(k) for k in bias], [float(v) for v in bias.values()]
-            if any(not 0 <= k < self.vocab for k in ids) or any(np.isnan(v) for v in vals):
-                raise ValueError("admit: a bias for a token outside the vocabulary, or that is no number")
+            if any(isinstance(k, (float, np.floating)) and k != i for k, i in zip(bias, ids)):
+                raise ValueError("admit: a bias for a token that is no whole number")
+            most = float(np.finfo(np.float32).max)
+            if any(not 0 <= k < self.vocab for k in ids) or any(not (abs(v) <= most or np.isinf(v)) for v in vals):
+                raise ValueError("admit: a bias for a token outside the vocabulary, or that is no number in fp32")
             f[i, 1:4], rec[i, 4] = pens, len(bias)
             rec[i, 6:6 + len(ids)], f[i, 6 + nb:6 + nb + len(ids)] = ids, vals
             if r.get("mask") is not None:

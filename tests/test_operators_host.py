@@ -1,10 +1,14 @@
 """What the operators' Python side does on the host: no GPU, the device's words are set by hand."""
 
+from types import SimpleNamespace
+
+import numpy as np
 import pytest
 import torch
 
 from cohere_inference_b200 import native as nv
 from cohere_inference_b200.packing import W8A8Linear
+from cohere_inference_b200.stream_decoder import StreamDecoder
 
 
 def test_w8a8_status_is_reported_once():
@@ -16,3 +20,27 @@ def test_w8a8_status_is_reported_once():
         lin.check_status()
     assert int(lin.status) == 0
     lin.check_status()
+
+
+def rule_tables(rules):
+    d = SimpleNamespace(vocab=20, max_bias=4, _rule_ints=6 + 2 * 4 + 1)
+    return StreamDecoder._rule_tables(d, list(range(len(rules))), rules)
+
+
+@pytest.mark.parametrize("rule", [
+    dict(repetition=1e-50), dict(repetition=1e39), dict(repetition=-1.0), dict(presence=1e39), dict(frequency=-1e39),
+    dict(bias={3: 1e39}), dict(bias={3: -3.5e38}), dict(bias={3.7: 1.0}), dict(bias={np.float32(0.5): 1.0}),
+])
+def test_rules_that_the_tables_cannot_hold_are_refused(rule):
+    with pytest.raises(ValueError):
+        rule_tables([rule])
+
+
+def test_rules_that_the_tables_hold():
+    rec = rule_tables([dict(repetition=1e-40, presence=3e38, frequency=-3e38, bias={3: np.inf, 4.0: -np.inf, "5": 3.4e38, np.int64(6): 1}),
+                       None, dict(repetition=np.float32(1.25), bias={})])
+    f = rec.view(np.float32)
+    assert rec[:, 0].tolist() == [0, 1, 2] and rec[:, 4].tolist() == [4, 0, 0] and rec[0, 6:10].tolist() == [3, 4, 5, 6]
+    assert np.array_equal(f[0, 1:4], np.array([1e-40, 3e38, -3e38], np.float32)) and f[0, 1] > 0
+    assert np.array_equal(f[0, 10:14], np.array([np.inf, -np.inf, 3.4e38, 1.0], np.float32))
+    assert f[1, 1:4].tolist() == [1.0, 0.0, 0.0] and f[2, 1:4].tolist() == [1.25, 0.0, 0.0]
