@@ -22,6 +22,15 @@ def test_w8a8_status_is_reported_once():
     lin.check_status()
 
 
+@pytest.mark.parametrize("raw", [None, lambda device: 100 + device])
+def test_stream_handle(monkeypatch, raw):
+    """With and without torch's undocumented way to the current stream's handle."""
+    monkeypatch.setattr(nv, "_raw_stream", raw)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: SimpleNamespace(cuda_stream=101))
+    assert nv.stream_ptr() == 101 and nv.stream_ptr(SimpleNamespace(cuda_stream=7)) == 7
+
+
 def rule_tables(rules):
     d = SimpleNamespace(vocab=20, max_bias=4, _rule_ints=6 + 2 * 4 + 1)
     return StreamDecoder._rule_tables(d, list(range(len(rules))), rules)
