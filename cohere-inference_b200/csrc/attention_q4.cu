@@ -512,6 +512,7 @@ int b200dec_attention_q4(int self, const int32_t* active, const float* q, int ld
   B200_REQUIRE((((uintptr_t)kcache | (uintptr_t)vcache) & 15) == 0 && ((uintptr_t)kpairs | (uintptr_t)vpairs) % (head_dim / 16) == 0 &&
                    (!sched || ((uintptr_t)sched & 15) == 0), "attention_q4: alignment");
   B200_REQUIRE(out_kind == B200DEC_OUT_F16 || out_kind == B200DEC_OUT_F32, "attention_q4: out_kind %d", out_kind);
+  B200_REQUIRE((uintptr_t)out % (out_kind == B200DEC_OUT_F16 ? 2 : 4) == 0, "attention_q4: alignment of out");
   Q4Args p{active, q, (uint8_t*)kcache, (uint8_t*)vcache, (uint32_t*)kpairs, (uint32_t*)vpairs, n, sched, out, part, count, status,
            ldq, heads, cap, slots, out_kind, cap, scale * 1.4426950408889634f};
   const int splits = part ? q4_splits(rows, heads, cap) : 1;

@@ -659,8 +659,9 @@ int b200dec_w8a8_prefill(const void* rows_image, const float* row_scale, int m, 
   B200_REQUIRE(m >= 1 && m <= MAX_MN && k >= 1 && k <= MAX_K8 && mode >= 1 && mode <= 3, "w8a8_prefill: m %d k %d mode %d", m, k, mode);
   B200_REQUIRE(pieces && n_pieces >= 1 && ck && cv && (mode == 1 || (ck_scale && cv_scale)), "w8a8_prefill: pieces and caches");
   B200_REQUIRE((((uintptr_t)rows_image | (uintptr_t)weight_image) & 1023) == 0 &&
-                   (((uintptr_t)w_scale | (uintptr_t)bias | (uintptr_t)pieces | (uintptr_t)ck | (uintptr_t)cv) & 15) == 0,
-               "w8a8_prefill: alignment (images 1 KB, the rest 16 bytes)");
+                   (((uintptr_t)w_scale | (uintptr_t)bias | (uintptr_t)pieces | (uintptr_t)ck | (uintptr_t)cv) & 15) == 0 &&
+                   (mode == 1 || (((uintptr_t)ck_scale | (uintptr_t)cv_scale) & 3) == 0),
+               "w8a8_prefill: alignment (images 1 KB, the caches' scales or pairs 4 bytes, the rest 16)");
   B200_REQUIRE((head_dim == 64 || head_dim == 128) && layers >= 1 && heads >= 1 && slots_plus_1 >= 1 && frames >= 1 &&
                    (int64_t)n == (int64_t)layers * 2 * heads * head_dim && n % BN == 0,
                "w8a8_prefill: n %d != layers %d x 2 x heads %d x head_dim %d (a multiple of 256)", n, layers, heads, head_dim);

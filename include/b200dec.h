@@ -373,11 +373,11 @@ int b200dec_scatter_kv_q8(const float* kv, const int32_t* slot_of, const int32_t
 /* b200dec_attention over 4-bit caches, for any cap: heads x head_dim as the caches have them, n[s] = 0 .. cap - 1 cached keys
  * (self != 0: the row's new key and value are written at n[s] and attended in this step as bf16 values) or 0 .. cap frames
  * (a row without any gives zeros). Scores, softmax and sums in fp32. sched: NULL, or a table of b200dec_row_schedule
- * (16-byte aligned; active, n and status are then not read). Alignment: q and the codes 16 bytes, pairs D / 16, ldq a multiple of
- * 4. part, count: a workspace of
- * b200dec_attention_q4_scratch_floats() floats and rows * heads counters, zero on entry and on exit, for the calls of one
- * stream at a time (two captured graphs that may run side by side need one each); both NULL: a row is one CTA however
- * long it is. Two rows of one call must not append to the same slot, the dummy excepted. */
+ * (16-byte aligned; active, n and status are then not read). Alignment: q and the codes 16 bytes, pairs D / 16, out that of its
+ * elements, ldq a multiple of 4. part, count: a workspace of b200dec_attention_q4_scratch_floats() floats and rows * heads
+ * counters, zero on entry and on exit, for the calls of one stream at a time (two captured graphs that may run side by side
+ * need one each); both NULL: a row is one CTA however long it is. Two rows of one call must not append to the same slot, the
+ * dummy excepted. */
 int b200dec_attention_q4(int self, const int32_t* active, const float* q, int ldq, void* kcache, void* vcache, void* kpairs,
                          void* vpairs, const int32_t* n, const int32_t* sched, int slots, int heads, int head_dim, int cap,
                          float scale, void* out, int out_kind, int rows, float* part, int32_t* count, int32_t* status, int pdl,
@@ -425,7 +425,7 @@ int b200dec_w8a8_linear(const void* rows_image, const float* row_scale, int m, i
                         const float* w_scale, const float* bias, int n, int act, void* out, int out_kind, int64_t ldo,
                         int32_t* status, void* stream);
 /* The same product into the slot caches: mode, pieces and caches as b200dec_prefill_gemm (mode 3: 4-bit caches, with their
- * pairs for ck_scale and cv_scale). */
+ * pairs for ck_scale and cv_scale; these 4-byte aligned). */
 int b200dec_w8a8_prefill(const void* rows_image, const float* row_scale, int m, int k, const void* weight_image,
                          const float* w_scale, const float* bias, int n, int mode, const int32_t* pieces, int n_pieces, void* ck,
                          void* cv, void* ck_scale, void* cv_scale, int layers, int slots_plus_1, int heads, int head_dim, int frames,

@@ -131,3 +131,13 @@ def test_w8a8_sizes(nv):
     assert lib.b200dec_w8a8_rows_bytes(1, 131073) == lib.b200dec_w8a8_weight_bytes(1, 131073) == -1
     refused(nv, lib.b200dec_w8a8_tile_weight(None, 4, 4, A, None), "1 KB")
     refused(nv, lib.b200dec_w8a8_tile_weight(A, 4, 4, A + 512, None), "1 KB")
+
+
+@pytest.mark.parametrize("change", [dict(out=A + 1), dict(out=A + 2, kind=1), dict(out=A + 3, kind=1)])
+def test_attention_q4_results_off_their_alignment(nv, change):
+    refused(nv, nv.lib().b200dec_attention_q4(*{**ATTEND, **change}.values()), "alignment of out")
+
+
+@pytest.mark.parametrize("change", [dict(mode=2, cks=A + 2), dict(mode=2, cvs=A + 1), dict(mode=3, cks=A + 2), dict(mode=3, cvs=A + 3)])
+def test_w8a8_prefill_scales_off_their_alignment(nv, change):
+    refused(nv, nv.lib().b200dec_w8a8_prefill(*{**PREFILL, **change}.values()), "alignment")
