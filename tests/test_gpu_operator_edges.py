@@ -1,16 +1,17 @@
 """Edges of the rules on the logits and of the 8-bit product: sizes of shared memory around the limit that needs no opt-in, slots without
-tokens, NaN through the activations, rows whose choice nobody takes."""
+tokens, NaN through the activations, rows whose choice nobody takes, a request's rules on their way through the scheduler."""
 
 import math
 import os
 import subprocess
 import sys
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
 import torch
 
-from cohere_inference_b200.synth import synthetic_model
+from cohere_inference_b200.synth import synthetic_model, synthetic_requests
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 sys.path.insert(0, HERE)
@@ -152,3 +153,33 @@ def test_w8a8_check_status(nv):
             lin.check_status()
     assert torch.equal(lin(x), y)
     lin.check_status()
+
+
+def test_rules_of_requests_reach_the_decoder(model16):
+    """Through DecodeScheduler: a banned token never comes, where it came without the ban, and penalised requests get the tokens that a
+    decoder gives which admits the same rules directly (steps of eight rows on both sides: a row's bits are its own)."""
+    from cohere_inference_b200.scheduler import DecodeScheduler
+    plain = [SimpleNamespace(**{**r.__dict__, "frames": min(r.frames, 60), "target": 20}) for r in synthetic_requests(12, seed=3)]
+    memory = lambda r: np.random.default_rng(r.frames).standard_normal((r.frames, 1024)).astype(np.float32)  # noqa: E731
+    new = lambda: decoder(model16, int8=True, logit_rules=True, buckets=(8,))  # noqa: E731
+    run = lambda rs: [np.asarray(x) for x in DecodeScheduler(new(), memory).run(rs)]  # noqa: E731
+    before = run(plain)
+    made = [t[len(r.prompt):] for t, r in zip(before, plain)]
+    rules = [dict(bias={int(v): -math.inf for v in set(made[i][::2].tolist())}) if i % 2 else dict(repetition=2.0 if i % 4 else 0.25)
+             for i in range(12)]
+    ruled = [SimpleNamespace(**{**r.__dict__, "rules": x}) for r, x in zip(plain, rules)]
+    got = run(ruled)
+    for i in range(1, 12, 2):
+        assert not set(got[i][len(plain[i].prompt):].tolist()) & set(rules[i]["bias"])
+    for i in range(0, 12, 2):
+        dec, n = new(), len(plain[i].prompt)
+        with torch.cuda.stream(dec.stream):
+            dec.fill_cross(torch.from_numpy(memory(plain[i])).cuda(), [plain[i].frames], [0])
+        dec.admit([0], [np.asarray(plain[i].prompt)], [plain[i].frames], [20], rules=[rules[i]])
+        b = dec.set_active([0])
+        for _ in range(n - 1 + 20):
+            dec.step(b)
+        dec.check_status()
+        assert np.array_equal(got[i], dec.out[0, :n + 20].cpu().numpy())
+    # some repeat themselves without a penalty, some do not: one of the two penalties shows
+    assert sum(not np.array_equal(got[i], before[i]) for i in range(0, 12, 2)) >= 3
