@@ -145,6 +145,12 @@ class DecodeScheduler:
         """Decode every request of the stream; returns the token arrays (prompt + generated) in request order.
         on_step(step_no, bucket, active slots) is called after each launch (used by the benchmark to time steps)."""
         dec, st = self.dec, self.stats
+        # rules that the decoder cannot take are refused before anything runs: half way they would take the other requests along
+        ruled = [r.rules for r in requests if getattr(r, "rules", None) is not None]
+        if ruled and not getattr(dec, "logit_rules", False):
+            raise ValueError("run: a request with rules needs a decoder made with logit_rules=True")
+        for rules in ruled:
+            dec.check_rules(rules)
         waiting = deque(sorted(range(len(requests)), key=lambda i: requests[i].arrival))
         results: list = [None] * len(requests)
         active: list[int] = []

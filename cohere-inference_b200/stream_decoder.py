@@ -760,6 +760,12 @@ class StreamDecoder:
             return m.view(np.int32)
         raise ValueError(f"mask: {self.vocab} booleans or {words} 32-bit words")
 
+    def check_rules(self, rules: dict | None) -> None:
+        """Raises ValueError where `admit` would refuse a request's rules."""
+        if not self.logit_rules:
+            raise ValueError("rules need a decoder made with logit_rules=True")
+        self._rule_tables([0], [rules])
+
     def _rule_tables(self, slots: list[int], rules: list[dict | None]) -> np.ndarray:
         """One record per request: slot, penalties, bias count, mask switch, bias ids, bias values, mask words."""
         rec = np.zeros((len(slots), self._rule_ints), np.int32)

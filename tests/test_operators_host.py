@@ -8,6 +8,7 @@ import torch
 
 from cohere_inference_b200 import native as nv
 from cohere_inference_b200.packing import W8A8Linear
+from cohere_inference_b200.scheduler import DecodeScheduler
 from cohere_inference_b200.stream_decoder import StreamDecoder
 
 
@@ -34,6 +35,31 @@ def test_stream_handle(monkeypatch, raw):
 def rule_tables(rules):
     d = SimpleNamespace(vocab=20, max_bias=4, _rule_ints=6 + 2 * 4 + 1)
     return StreamDecoder._rule_tables(d, list(range(len(rules))), rules)
+
+
+class Decoder:
+    """As much of a decoder as a run looks at before its first request; a call that starts one fails the test."""
+    slots, max_new_tokens, eos = 3, 8, -1
+    vocab, max_bias, _rule_ints = 20, 4, 6 + 2 * 4 + 1
+    check_rules, _rule_tables, _mask_words = StreamDecoder.check_rules, StreamDecoder._rule_tables, StreamDecoder._mask_words
+
+    def __init__(self, logit_rules):
+        self.logit_rules, self.out = logit_rules, np.zeros((4, 12), np.int64)
+
+    def fill_cross(self, *args):
+        raise AssertionError("a request was started")
+
+    admit = set_active = step = fill_cross
+
+
+@pytest.mark.parametrize("logit_rules, rules", [(False, dict(repetition=2.0)), (True, dict(repetition=-2.0)), (True, dict(mask=np.ones(19, bool)))])
+def test_a_run_refuses_rules_before_it_starts(logit_rules, rules):
+    """The last request's rules are refused before the first is admitted, and the scheduler keeps its slots."""
+    request = lambda **kw: SimpleNamespace(prompt=[1, 2], frames=5, target=4, arrival=0.0, **kw)  # noqa: E731
+    sched = DecodeScheduler(Decoder(logit_rules), lambda r: np.zeros((r.frames, 4), np.float32))
+    with pytest.raises(ValueError):
+        sched.run([request(), request(rules=None), request(rules=rules)])
+    assert sorted(sched.free) == [0, 1, 2] and sched.stats.admitted == 0
 
 
 @pytest.mark.parametrize("rule", [
