@@ -1,9 +1,11 @@
-// The 4-bit cache format, shared by everything that writes it (kv4.cu, attention_q4.cu, prefill_gemm.cu).
+// The 4-bit cache format, shared by everything that writes it (kv4.cu, attention_q4.cu, prefill_gemm.cu, w8a8.cu).
 //
 // A head vector is rounded to bf16 (what the bf16 cache would hold), clamped to +-32752 with NaN as 0, and cut into groups of
 // 64 dims. Per group: lo = fp16(min), step = fp16((max - lo) / 15), code = clamp(rint((x - lo) / step), 0, 15), 0 where step
-// is 0; x ~ lo + code * step. Within half a step, except that rounding lo and step to 11 bits can move a value by
-// 2^-12 (|lo| + range) more. The clamp keeps max - min inside fp16. 64 dims share a (step, lo) pair of 4 bytes: 4.5 bits a value.
+// is 0; x ~ lo + code * step, and x is within half a step of that. fp16 holds a bf16 value as it is down to 2^-14, so lo is
+// exact, and a step that is off by 2^-11 of itself moves the fifteenth code by less than a hundredth of a step. Below 2^-14
+// fp16 numbers are 2^-24 apart: a lo there is off by up to 2^-25, a step by as much, fifteen times over at the top, and together
+// that is up to 2^-21 more. The clamp keeps max - min inside fp16. 64 dims share a (step, lo) pair of 4 bytes: 4.5 bits a value.
 // A vector's codes are D / 2 bytes, dim 2i in the low half of byte i; its pairs are D / 64 half2 {step, lo}.
 #pragma once
 #include "common.cuh"

@@ -79,3 +79,19 @@ def test_rules_that_the_tables_hold():
     assert np.array_equal(f[0, 1:4], np.array([1e-40, 3e38, -3e38], np.float32)) and f[0, 1] > 0
     assert np.array_equal(f[0, 10:14], np.array([np.inf, -np.inf, 3.4e38, 1.0], np.float32))
     assert f[1, 1:4].tolist() == [1.0, 0.0, 0.0] and f[2, 1:4].tolist() == [1.25, 0.0, 0.0]
+
+
+def test_how_far_the_4_bit_format_is_off():
+    """Half a step; 2^-21 more where the step or the lowest value is below fp16's normal numbers. In 64 bits, from the definition."""
+    rng = np.random.default_rng(0)
+    off, spread = (10.0 ** rng.uniform(-9, 4.5, (2, 4000, 1)))
+    x = torch.from_numpy(rng.choice([-1.0, 0.0, 1.0], (4000, 1)) * off + spread * rng.standard_normal((4000, 64)))
+    x[0], x[1], x[2, 1:] = 3.7, -2.0 ** -20, x[2, 0]  # constant groups
+    x = x.clamp(-32752.0, 32752.0).bfloat16().double()
+    lo = x.amin(1, keepdim=True).half().double()
+    step = ((x.amax(1, keepdim=True) - lo) / 15).half().double()
+    code = torch.where(step > 0, ((x - lo) / torch.where(step > 0, step, 1.0)).round().clamp(0, 15), 0.0)
+    far = (lo + code * step - x).abs() - step.abs() / 2
+    normal = ((step >= 2.0 ** -14) & (lo.abs() >= 2.0 ** -14)).flatten()
+    assert normal.sum() > 500 and (~normal).sum() > 500
+    assert far[normal].max() <= 0 and far.max() <= 2.0 ** -21
