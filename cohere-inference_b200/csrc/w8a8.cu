@@ -8,7 +8,8 @@
 //   * persistent CTAs walk the (channel tile, row tile) list: warp 0 feeds the ring, warp 1 issues the MMAs into one of two
 //     accumulators, warps 2-17 drain the other: four warps per 32 lanes, each a quarter of the tile's columns. Per k the MMA is
 //     twice as fast as with 16-bit operands, so the epilogue decides, and what decides it is latency: 13 600 x 1024 x 16 384 to bf16
-//     took 591 us with four warps, 258-274 with eight, 240 with sixteen and turned stores; the products alone take 152 us (the slope over k).
+//     took 591 us with four warps, 258-274 with eight, 218-240 with sixteen and turned stores (k = 128: 232 with eight, 147 with
+//     sixteen); the products alone take 135 us (the slope from k = 1024 to 2048).
 //     Pairs of CTAs (cta_group::2), which copy a third less, were slower: 390 us per 1024 of k.
 //   * channel scales and biases of a tile go to shared memory once, as pairs, and are read back as broadcasts.
 //   * rows leave in runs of 64 bytes; rows that are not 16-byte aligned through a transposition in shared memory.
